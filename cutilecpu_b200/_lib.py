@@ -21,6 +21,61 @@ MK_ERR_DEVICE_FAULT = -5
 MK_F = {"identity": 0, "abs2": 1, "abs": 2, "gt0": 3}
 MK_OP = {"add": 0, "max": 1, "min": 2, "mul": 3}
 
+MK_T = {"Float32": 0, "Float16": 1, "BFloat16": 2}
+MK_ACT = {"silu": 0, "sigmoid": 1}
+MK_SCAN_PIECE = 64
+
+
+# Argument structs of the state space operators, fields as in the header.
+class ConvArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("type", "width", "silu")] + \
+        [(n, C.c_int64) for n in ("D", "T", "nseq", "len")] + \
+        [("seqs", C.c_void_p), ("slots", C.c_void_p), ("nslots", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64),
+         ("y", C.c_void_p), ("ldy", C.c_int64), ("w", C.c_void_p), ("bias", C.c_void_p), ("init", C.c_void_p),
+         ("last", C.c_void_p), ("dy", C.c_void_p), ("lddy", C.c_int64), ("dlast", C.c_void_p), ("dx", C.c_void_p),
+         ("lddx", C.c_int64), ("dw", C.c_void_p), ("dbias", C.c_void_p), ("dinit", C.c_void_p),
+         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class ConvStepArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("type", "width", "silu")] + \
+        [("D", C.c_int64), ("B", C.c_int64), ("slots", C.c_void_p), ("nslots", C.c_int64), ("x", C.c_void_p),
+         ("ldx", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("state", "next", "w", "bias")]
+
+
+class ScanArgs(C.Structure):
+    _fields_ = [("type", C.c_int32), ("softplus", C.c_int32)] + \
+        [(n, C.c_int64) for n in ("D", "N", "G", "T", "nseq", "len")] + \
+        [("seqs", C.c_void_p), ("slots", C.c_void_p), ("nslots", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("u", "delta", "z", "B", "C")] + \
+        [(n, C.c_int64) for n in ("ldu", "lddelta", "ldz", "ldb", "ldc")] + \
+        [(n, C.c_void_p) for n in ("A", "Dskip", "bias", "init", "y")] + \
+        [("ldy", C.c_int64), ("last", C.c_void_p), ("saved", C.c_void_p), ("dy", C.c_void_p), ("lddy", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("dlast", "du", "ddelta", "dz", "dB", "dC")] + \
+        [(n, C.c_int64) for n in ("lddu", "ldddelta", "lddz", "lddb", "lddc")] + \
+        [(n, C.c_void_p) for n in ("dA", "dDskip", "dbias", "dinit", "workspace")] + \
+        [("workspace_bytes", C.c_size_t)]
+
+
+class ScanStepArgs(C.Structure):
+    _fields_ = [("type", C.c_int32), ("softplus", C.c_int32)] + \
+        [(n, C.c_int64) for n in ("D", "N", "G", "B")] + [("slots", C.c_void_p), ("nslots", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("u", "delta", "z", "Bmat", "Cmat")] + \
+        [(n, C.c_int64) for n in ("ldu", "lddelta", "ldz", "ldb", "ldc")] + \
+        [(n, C.c_void_p) for n in ("A", "Dskip", "bias", "state", "next", "y")] + [("ldy", C.c_int64)]
+
+
+class NormArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("type", "rtype", "act")] + [("eps", C.c_float)] + \
+        [("D", C.c_int64), ("T", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("r", "h", "gate", "hw", "scale", "w", "rout", "y")] + \
+        [(n, C.c_int64) for n in ("ldr", "ldh", "ldgate", "ldrout", "ldy")] + \
+        [(n, C.c_void_p) for n in ("dy", "drout", "dr", "dh", "dgate", "dhw", "dscale", "dw")] + \
+        [(n, C.c_int64) for n in ("lddy", "lddrout", "lddr", "lddh", "lddgate")] + \
+        [("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 # name -> (restype, argtypes); keep in step with include/mk_kernels.h
 _i64, _i32, _f64, _vp, _int = C.c_int64, C.c_int32, C.c_double, C.c_void_p, C.c_int
 SIGNATURES = {
@@ -55,6 +110,18 @@ SIGNATURES = {
     "mk_hist_u32_allreduce": (_int, [_vp, _vp, _i32, _vp, _i64, _vp]),
     "mk_hist_u32_allreduce_async": (_int, [_vp, _vp, _i32, _vp, _i64, _vp]),
     "mk_hist_allreduce_complete": (_int, [_vp]),
+    "mk_causal_conv": (_int, [C.POINTER(ConvArgs), _vp]),
+    "mk_causal_conv_grad_workspace": (_int, [C.POINTER(ConvArgs), C.POINTER(C.c_size_t)]),
+    "mk_causal_conv_grad": (_int, [C.POINTER(ConvArgs), _vp]),
+    "mk_causal_conv_step": (_int, [C.POINTER(ConvStepArgs), _vp]),
+    "mk_selective_scan_workspace": (_int, [C.POINTER(ScanArgs), C.POINTER(C.c_size_t)]),
+    "mk_selective_scan": (_int, [C.POINTER(ScanArgs), _vp]),
+    "mk_selective_scan_grad_workspace": (_int, [C.POINTER(ScanArgs), C.POINTER(C.c_size_t)]),
+    "mk_selective_scan_grad": (_int, [C.POINTER(ScanArgs), _vp]),
+    "mk_selective_scan_step": (_int, [C.POINTER(ScanStepArgs), _vp]),
+    "mk_block_norm": (_int, [C.POINTER(NormArgs), _vp]),
+    "mk_block_norm_grad_workspace": (_int, [C.POINTER(NormArgs), C.POINTER(C.c_size_t)]),
+    "mk_block_norm_grad": (_int, [C.POINTER(NormArgs), _vp]),
     "mk_pool_alloc_device": (_int, [C.POINTER(C.c_void_p), C.c_size_t, _vp]),
     "mk_pool_free_device": (_int, [_vp, _vp]),
     "mk_host_alloc_aligned": (_int, [C.POINTER(C.c_void_p), C.c_size_t, C.c_size_t]),

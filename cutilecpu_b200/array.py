@@ -22,19 +22,23 @@ import torch
 from . import _lib
 
 # Julia element type name -> (numpy dtype, torch storage dtype).  UInt32 is
-# stored in an int32 tensor and reinterpreted bit-for-bit on the host.
+# stored in an int32 tensor and reinterpreted bit-for-bit on the host.  numpy
+# has no BFloat16: host copies are float32, exact one way and rounded to the
+# nearest the other.
 ELTYPES = {
     "Float32": (np.dtype(np.float32), torch.float32),
     "Float64": (np.dtype(np.float64), torch.float64),
     "Int32": (np.dtype(np.int32), torch.int32),
     "UInt32": (np.dtype(np.uint32), torch.int32),
     "Int64": (np.dtype(np.int64), torch.int64),
+    "Float16": (np.dtype(np.float16), torch.float16),
+    "BFloat16": (np.dtype(np.float32), torch.bfloat16),
 }
 _BY_NUMPY = {np.dtype(np.float32): "Float32", np.dtype(np.float64): "Float64",
              np.dtype(np.int32): "Int32", np.dtype(np.uint32): "UInt32",
-             np.dtype(np.int64): "Int64"}
+             np.dtype(np.int64): "Int64", np.dtype(np.float16): "Float16"}
 _BY_TORCH = {torch.float32: "Float32", torch.float64: "Float64", torch.int32: "Int32",
-             torch.int64: "Int64"}
+             torch.int64: "Int64", torch.float16: "Float16", torch.bfloat16: "BFloat16"}
 
 
 def eltype_name(T) -> str:
@@ -149,13 +153,63 @@ class MLIRArray:
 
     def to_numpy(self) -> np.ndarray:
         """``Array(a)``: a host copy with Julia dims, Fortran order."""
-        host = self.storage.detach().cpu().numpy()
+        t = self.storage.detach().cpu()
+        host = (t.float() if self.eltype == "BFloat16" else t).numpy()
         if self.eltype == "UInt32":
             host = host.view(np.uint32)
         return host.reshape(self.dims, order="F")
 
     def __repr__(self) -> str:
         return f"MLIRArray{{{self.eltype},{len(self.dims)}}}(dims={self.dims}, device=cuda:{self.device})"
+
+
+class MLIRRows:
+    """``@view A[lo:hi, :]`` of an MLIRArray (1-based, inclusive): neighbouring
+    rows of every column, without a copy; columns stay ``ld`` elements apart.
+    The operators over token columns take it where they take an MLIRArray, so a
+    projection's parts need not be copied out of its result."""
+
+    __slots__ = ("parent", "storage", "dims", "eltype", "ld")
+
+    def __init__(self, parent: MLIRArray, lo: int, hi: int):
+        if not isinstance(parent, MLIRArray) or parent.ndims < 2:
+            raise TypeError("rows: expected an MLIRArray of two or more dimensions")
+        if not 1 <= lo <= hi + 1 or hi > parent.dims[0]:
+            raise IndexError(f"rows {lo}:{hi} out of bounds for {parent.dims[0]} rows")
+        self.parent, self.eltype, self.ld = parent, parent.eltype, parent.dims[0]
+        self.dims = (hi - lo + 1,) + parent.dims[1:]
+        self.storage = parent.storage[lo - 1:]
+
+    @property
+    def shape(self) -> tuple[int, ...]:
+        return self.dims
+
+    @property
+    def ndims(self) -> int:
+        return len(self.dims)
+
+    @property
+    def length(self) -> int:
+        return math.prod(self.dims)
+
+    @property
+    def device(self) -> int:
+        return self.storage.device.index
+
+    def pointer(self) -> int:
+        return self.storage.data_ptr()
+
+    def to_numpy(self) -> np.ndarray:
+        lo = self.parent.storage.numel() - self.storage.numel()
+        return self.parent.to_numpy()[lo:lo + self.dims[0]]
+
+    def __repr__(self) -> str:
+        return f"MLIRRows{{{self.eltype}}}(dims={self.dims}, ld={self.ld}, device=cuda:{self.device})"
+
+
+def rows(a: MLIRArray, lo: int, hi: int) -> MLIRRows:
+    """``@view a[lo:hi, :]`` (1-based, inclusive)."""
+    return MLIRRows(a, lo, hi)
 
 
 def Array(a: MLIRArray) -> np.ndarray:
@@ -231,7 +285,7 @@ def on_device(*arrays):
     current (the library launches on the current device and its current
     stream), after checking that they all live on the same device."""
     import contextlib
-    devs = {a.device for a in arrays if isinstance(a, MLIRArray)}
+    devs = {a.device for a in arrays if isinstance(a, (MLIRArray, MLIRRows))}
     if len(devs) > 1:
         raise _lib.MLIRKernelsError(f"MLIRCUDABackend: arguments live on different devices {sorted(devs)}")
     if not devs or next(iter(devs)) == torch.cuda.current_device():

@@ -225,6 +225,8 @@ int mk_error_poll(void* stream) {
   std::string msg = "device fault:";
   if (word & mk::ERRBIT_GATHER_INDEX) msg += " gather index out of bounds;";
   if (word & mk::ERRBIT_HIST_KEY) msg += " histogram key out of range;";
+  if (word & mk::ERRBIT_SEQS) msg += " sequence offsets out of order or out of range;";
+  if (word & mk::ERRBIT_SLOT) msg += " state slot out of range or used twice;";
   if (word & mk::ERRBIT_TIMEOUT) {
     msg += " bounded device wait timed out;";
     mk::fail(MK_ERR_TIMEOUT, msg);

@@ -16,6 +16,8 @@ enum : unsigned {
   ERRBIT_GATHER_INDEX = 1u << 0,  // gather index outside [1, na]
   ERRBIT_HIST_KEY = 1u << 1,      // histogram key outside [1, nbins]
   ERRBIT_TIMEOUT = 1u << 2,       // a bounded device wait gave up
+  ERRBIT_SEQS = 1u << 3,          // sequence offsets that descend or leave the columns
+  ERRBIT_SLOT = 1u << 4,          // state slot above the pool, or used twice in one call
 };
 
 // Per-device state, created once under a mutex (api.cu).

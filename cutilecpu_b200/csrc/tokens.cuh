@@ -1,0 +1,221 @@
+// tokens.cuh — shared by the kernels over token columns (causal_conv.cu,
+// selective_scan.cu, block_norm.cu): element types, the packed sequences of a
+// (channels, tokens) matrix, and the scalar functions of their formulas.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "mk_common.cuh"
+
+namespace mk {
+namespace tok {
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// V neighbouring elements as one access, or as several of 16 bytes.
+template <typename T, int V> struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Vec { T v[V]; };
+
+template <typename T, int V>
+__device__ __forceinline__ void load(float (&f)[V], const T* p) {
+  const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = to_f(v.v[i]);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const float (&f)[V]) {
+  Vec<T, V> v;
+#pragma unroll
+  for (int i = 0; i < V; ++i) v.v[i] = from_f<T>(f[i]);
+  *reinterpret_cast<Vec<T, V>*>(p) = v;
+}
+
+// Packed sequences.  With `seqs` sequence s has the columns
+// [seqs[s] - 1, seqs[s + 1] - 1) (1-based offsets, as Julia ranges start);
+// without it every sequence has `len` columns.  Offsets live on the device,
+// so they are read defensively: a sequence that does not lie inside the T
+// columns, or ends before it begins, counts as empty and sets `bad`.
+struct Seqs {
+  const int32_t* seqs;
+  int64_t nseq, len, T;
+};
+
+struct Span {
+  int64_t lo, hi;
+  bool bad;
+};
+
+__device__ __forceinline__ int64_t seq_offset(const Seqs& q, int64_t s) {
+  if (!q.seqs) return s * q.len;
+  int64_t o = (int64_t)q.seqs[s] - 1;
+  return o < 0 ? 0 : (o > q.T ? q.T : o);
+}
+
+__device__ __forceinline__ Span seq_span(const Seqs& q, int64_t s) {
+  if (!q.seqs) return {s * q.len, (s + 1) * q.len, false};
+  const int64_t lo = (int64_t)q.seqs[s] - 1, hi = (int64_t)q.seqs[s + 1] - 1;
+  const bool bad = lo < 0 || hi > q.T || hi < lo;
+  const int64_t at = lo < 0 ? 0 : (lo > q.T ? q.T : lo);
+  return {at, bad ? at : hi, bad};
+}
+
+// A sequence cut into pieces of `piece` columns (the last one shorter): piece
+// c of sequence s has the number lo(s) / piece + s + c.  The numbers of
+// sequence s + 1 begin behind those of s, because floor(a + b) >= floor(a) +
+// floor(b); all lie below T / piece + nseq, so no prefix sum over the
+// sequences is needed to place per-piece state.
+__device__ __forceinline__ int64_t first_piece(const Seqs& q, int64_t s, int64_t piece) {
+  return seq_offset(q, s) / piece + s;
+}
+
+// The sequence that piece number `i` falls to (the last s with first_piece <= i).
+__device__ __forceinline__ int64_t seq_of_piece(const Seqs& q, int64_t i, int64_t piece) {
+  int64_t lo = 0, hi = q.nseq - 1;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi + 1) >> 1;
+    if (first_piece(q, mid, piece) <= i) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Row of the state pool that entry i uses: slots[i] - 1, or i without slots.
+// -1: none (slots[i] <= 0); a slot above nslots counts as none and is flagged.
+__device__ __forceinline__ int64_t slot_of(const int32_t* slots, int64_t nslots, int64_t i, unsigned* err) {
+  if (!slots) return i;
+  const int64_t k = (int64_t)slots[i] - 1;
+  if (k >= nslots) {
+    atomicOr(err, ERRBIT_SLOT);
+    return -1;
+  }
+  return k < 0 ? -1 : k;
+}
+
+// Two entries of one call on one slot would race on its state: entry i is
+// compared with those before it by the `nt` threads of a block (the caller
+// picks one block per entry), and a repeat is flagged.
+__device__ __forceinline__ void check_distinct(const int32_t* slots, int64_t i, int tid, int nt, unsigned* err) {
+  if (!slots || slots[i] <= 0) return;
+  const int32_t mine = slots[i];
+  bool twice = false;
+  for (int64_t j = tid; j < i; j += nt) twice |= slots[j] == mine;
+  if (twice) atomicOr(err, ERRBIT_SLOT);
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// 2^x by the special function unit (relative error about 2^-22).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + expf(-x)); }
+
+// log(1 + e^x) = max(x, 0) + log1p(e), e = e^-|x| in (0, 1].  log1p(e) =
+// 2 artanh(s), s = e / (2 + e) <= 1/3: eight terms of the series leave less
+// than 2^-26 relative, so small steps (large negative x) keep full precision,
+// which log(1 + e) in 32 bits loses.
+__device__ __forceinline__ float softplus(float x) {
+  const float e = expf(-fabsf(x));
+  const float s = __fdividef(e, 2.0f + e), w = s * s;
+  float p = 1.0f / 15.0f;
+  p = fmaf(p, w, 1.0f / 13.0f);
+  p = fmaf(p, w, 1.0f / 11.0f);
+  p = fmaf(p, w, 1.0f / 9.0f);
+  p = fmaf(p, w, 1.0f / 7.0f);
+  p = fmaf(p, w, 1.0f / 5.0f);
+  p = fmaf(p, w, 1.0f / 3.0f);
+  p = fmaf(p * w, s, s);
+  return fmaf(2.0f, p, fmaxf(x, 0.0f));
+}
+
+// The sums of v[0..7] over the R lanes that differ in r (lane distance
+// STRIDE), scattered: for R <= 8 lane r ends with the sums of values e * R + r
+// (out[e], e < 8 / R); for R > 8 lanes with equal r % 8 all hold value r % 8.
+// Each stage sends half of what is left, so 8 sums over 8 lanes take 7
+// shuffles instead of 24.  The order of the additions is fixed.
+template <int R, int STRIDE>
+__device__ __forceinline__ void reduce_scatter8(float (&v)[8], int r, float (&out)[R < 8 ? 8 / R : 1]) {
+  constexpr int W = R < 8 ? R : 8;
+  constexpr int E = 8 / W;
+#pragma unroll
+  for (int bit = W / 2; bit >= 1; bit /= 2) {
+    const bool up = (r & bit) != 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+      for (int q = 0; q < bit; ++q) {
+        const float lo = v[e * W + q], hi = v[e * W + bit + q];
+        const float keep = up ? hi : lo, send = up ? lo : hi;
+        v[e * W + q] = keep + __shfl_xor_sync(0xffffffffu, send, bit * STRIDE);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+#pragma unroll
+    for (int bit = 8; bit < R; bit *= 2) v[e * W] += __shfl_xor_sync(0xffffffffu, v[e * W], bit * STRIDE);
+    out[e] = v[e * W];
+  }
+}
+
+// Runs a C entry point's body: no C++ exception leaves it.
+template <typename F>
+inline int guarded(F&& f) {
+  try {
+    return f();
+  } catch (...) {
+    return MK_ERR_INVALID;
+  }
+}
+
+inline size_t type_bytes(int type) { return type == MK_T_F32 ? 4 : 2; }
+
+// Host-side checks shared by the entry points.
+inline bool elem_aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// Whether a matrix at p with this leading dimension can be read V elements of es bytes at a time.
+inline bool vec_ok(const void* p, int64_t ld, size_t es, int V) {
+  const int64_t n = (int64_t)es * V < 16 ? (int64_t)es * V : 16;
+  return reinterpret_cast<uintptr_t>(p) % n == 0 && (ld * (int64_t)es) % n == 0;
+}
+
+inline int bad(const char* who, const std::string& what) {
+  return fail(MK_ERR_INVALID, std::string(who) + ": " + what);
+}
+
+// A matrix of `cols` columns of `rows` elements: there where it has elements, aligned, ld >= rows.
+inline int check_matrix(const char* who, const char* name, const void* p, int64_t rows, int64_t ld, int64_t cols,
+                        size_t es) {
+  if (cols == 0) return MK_OK;
+  if (!p) return bad(who, std::string(name) + " is null");
+  if (ld < rows) return bad(who, std::string(name) + " has a leading dimension below its rows");
+  if (!elem_aligned(p, es)) return bad(who, std::string(name) + " is not element-aligned");
+  return MK_OK;
+}
+
+// Float32 parameters and states; `vec`: read as 16-byte vectors.
+inline int check_floats(const char* who, const char* name, const void* p, bool required, bool vec) {
+  if (!p) return required ? bad(who, std::string(name) + " is null") : MK_OK;
+  if (!elem_aligned(p, vec ? 16 : 4))
+    return bad(who, std::string(name) + (vec ? " is not 16-byte aligned" : " is not 4-byte aligned"));
+  return MK_OK;
+}
+
+}  // namespace tok
+}  // namespace mk
+
+#define MK_TRY(x)                 \
+  do {                            \
+    const int rc_ = (x);          \
+    if (rc_ != MK_OK) return rc_; \
+  } while (0)

@@ -45,14 +45,18 @@ def pool_allocate(T, dims) -> MLIRArray:
     d = _dims(dims)
     n = math.prod(d)
     npdt, tdt = ELTYPES[name]
-    nbytes = max(1, n) * npdt.itemsize
+    itemsize = torch.empty(0, dtype=tdt).element_size()
+    nbytes = max(1, n) * itemsize
     p = C.c_void_p()
     stream = current_stream_handle()
     _lib.check(_lib.lib().mk_pool_alloc_device(C.byref(p), nbytes, stream), "pool_allocate")
-    typestr = np.dtype(np.int32 if name == "UInt32" else npdt).str
+    # BFloat16 has no array-interface type: exposed as 16-bit integers and viewed
+    typestr = np.dtype({"UInt32": np.int32, "BFloat16": np.int16}.get(name, npdt)).str
     block = _DeviceBlock(p.value, nbytes, typestr, (n,), stream)
     t = torch.as_tensor(block, device="cuda")
     assert t.data_ptr() == p.value, "pool_allocate: torch copied the block"
+    if name == "BFloat16":
+        t = t.view(tdt)
     weakref.finalize(t, _free_device, p.value, stream)
     return MLIRArray(t, dims=d, eltype=name)
 
@@ -78,6 +82,8 @@ def _free_host(ptr: int) -> None:
 def aligned_array(T, dims, alignment: int = 64) -> np.ndarray:
     """A pinned host array whose data pointer is ``alignment``-aligned."""
     _check_alignment(alignment)
+    if eltype_name(T) == "BFloat16":
+        raise TypeError("aligned_array: numpy has no BFloat16")
     npdt = ELTYPES[eltype_name(T)][0]
     d = _dims(dims)
     nbytes = max(1, math.prod(d)) * npdt.itemsize

@@ -294,6 +294,223 @@ MK_API int mk_hist_allreduce_complete(void* stream);
  * entries = 0 turns it off.  Needs the mailbox (mk_peer_create). */
 MK_API int mk_peer_trace(unsigned long long* log_dev, int entries);
 
+/* ---- state space operators ------------------------------------------------
+ * Operators over (channels, tokens) matrices, column-major: a token's channels
+ * are contiguous, `ld*` elements apart from the next token's, so row ranges of
+ * a wider matrix (a projection's parts) are passed without a copy.  They stand
+ * beside mk_accumulate_f32 and mk_mapreduce_dim_f32, which the reference's
+ * AK.accumulate! and mapreducedim! cover, and have no counterpart there.
+ *
+ * Element types of the token matrices: MK_T_*.  Parameters (w, bias, A, ...)
+ * and their gradients are Float32; sums and states are kept in Float32.
+ *
+ * Sequences: with seqs (nseq + 1 offsets on the device, 1-BASED, ascending),
+ * sequence s has the columns seqs[s] .. seqs[s+1]-1; columns outside all
+ * sequences are neither read nor written.  With seqs == NULL every sequence
+ * has `len` columns and nseq * len == T.  A sequence may be empty; its state
+ * passes through.  Offsets that descend or leave the T columns make that
+ * sequence empty and set the device error word (mk_error_poll).
+ * Slots: with slots (one 1-BASED Int32 per sequence or batch entry), the
+ * state of entry i is column slots[i] of the pool; slots[i] <= 0 means none
+ * (a prompt then starts from zero and leaves no state; a step's entry is
+ * padding: neither its y nor a state is written).  A slot above nslots, or one
+ * that two entries share, sets the error word (an entry whose slot is above
+ * nslots is treated as having none; what a shared slot holds is undefined).
+ *
+ * None of them allocates: what a call needs is a workspace of the size that
+ * the *_workspace function gives, owned by the caller, free for other use once
+ * the call's work on the stream is done.  Matrices that are written must not
+ * overlap others unless said so below.  Results do not depend on timing
+ * (no floating-point atomics). */
+#define MK_T_F32  0
+#define MK_T_F16  1
+#define MK_T_BF16 2
+
+#include <stddef.h>
+
+/* Causal convolution of each channel with W = width taps (2 to 4):
+ *   pre[d,t] = bias[d] + sum_{k=1..W} w[d,k] x[d,t-W+k],  y = silu ? pre*sigmoid(pre) : pre
+ * where x before a sequence's first column is its state (D, W-1 columns, the
+ * oldest first) or zero.  w is (D, W) column-major.  `last` receives the last
+ * W-1 columns of [state | x]; it may be `init` itself.
+ * The gradient takes dy and, optionally, dlast, and writes dx, dw, dbias and
+ * dinit (where not NULL): those of w and bias summed over all tokens. */
+typedef struct mk_conv_args {
+  int32_t type;                 /* MK_T_* of x, y, dy, dx and the states      */
+  int32_t width;                /* W                                          */
+  int32_t silu;                 /* 0: y = pre                                 */
+  int64_t D, T, nseq, len;
+  const int32_t* seqs;
+  const int32_t* slots;         /* forward only */
+  int64_t nslots;
+  const void* x;
+  int64_t ldx;
+  void* y;                      /* forward; not x */
+  int64_t ldy;
+  const float* w;
+  const float* bias;            /* D, or NULL */
+  const void* init;             /* (D, W-1, nseq or nslots), or NULL */
+  void* last;                   /* forward, or NULL */
+  /* gradient */
+  const void* dy;
+  int64_t lddy;
+  const void* dlast;            /* (D, W-1, nseq), or NULL */
+  void* dx;                     /* not x, not dy */
+  int64_t lddx;
+  float* dw;                    /* (D, W) */
+  float* dbias;                 /* D, or NULL */
+  void* dinit;                  /* (D, W-1, nseq), or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+} mk_conv_args;
+MK_API int mk_causal_conv(const mk_conv_args* args, void* stream);
+MK_API int mk_causal_conv_grad_workspace(const mk_conv_args* args, size_t* bytes);
+MK_API int mk_causal_conv_grad(const mk_conv_args* args, void* stream);
+
+/* One token per batch entry: y from [state | x], and next = the state moved on
+ * by x (next may be state itself). */
+typedef struct mk_conv_step_args {
+  int32_t type, width, silu;
+  int64_t D, B;
+  const int32_t* slots;
+  int64_t nslots;
+  const void* x;
+  int64_t ldx;
+  void* y;
+  int64_t ldy;
+  const void* state;            /* (D, W-1, B or nslots) */
+  void* next;
+  const float* w;
+  const float* bias;
+} mk_conv_step_args;
+MK_API int mk_causal_conv_step(const mk_conv_step_args* args, void* stream);
+
+/* Selective state space scan.  Per channel d of group g (D/G neighbouring
+ * channels share the columns of B and C) and state n, along a sequence:
+ *   dt = softplus ? log(1 + exp(delta + bias)) : delta + bias
+ *   h[n] = exp(dt * A[n,d]) * h[n] + dt * u * B[n,g,t]
+ *   y = (sum_n C[n,g,t] * h[n] + Dskip[d] * u) * (z ? z*sigmoid(z) : 1)
+ * A is (N, D), states are (N, D, sequence) Float32, B and C have G*N rows
+ * (n fastest).  1 <= N <= 64.  h starts at init (or zero); `last` receives the
+ * final h and may be `init` itself.  y may be u, delta or z (same ld).
+ * `saved`, when not NULL, receives the states at the start of every piece of
+ * MK_SCAN_PIECE columns: (N, D, T/MK_SCAN_PIECE + nseq) Float32; the gradient
+ * needs it.
+ * The gradient takes dy and, optionally, dlast, and writes du, ddelta, dB, dC,
+ * dA, and those of the other inputs that are given (dz, dDskip, dbias: not
+ * NULL exactly when z, Dskip, bias are; dinit optional). */
+#define MK_SCAN_PIECE 64
+typedef struct mk_scan_args {
+  int32_t type;                 /* MK_T_* of u, delta, z, B, C, y and their gradients */
+  int32_t softplus;
+  int64_t D, N, G, T, nseq, len;
+  const int32_t* seqs;
+  const int32_t* slots;         /* forward only */
+  int64_t nslots;
+  const void* u;
+  const void* delta;
+  const void* z;                /* or NULL */
+  const void* B;
+  const void* C;
+  int64_t ldu, lddelta, ldz, ldb, ldc;
+  const float* A;
+  const float* Dskip;           /* D, or NULL */
+  const float* bias;            /* D, or NULL */
+  const float* init;            /* or NULL */
+  void* y;                      /* forward */
+  int64_t ldy;
+  float* last;                  /* forward, or NULL */
+  float* saved;                 /* written forward (or NULL), read by the gradient */
+  /* gradient */
+  const void* dy;
+  int64_t lddy;
+  const float* dlast;           /* or NULL */
+  void* du;
+  void* ddelta;
+  void* dz;
+  void* dB;
+  void* dC;
+  int64_t lddu, ldddelta, lddz, lddb, lddc;
+  float* dA;
+  float* dDskip;
+  float* dbias;
+  float* dinit;                 /* or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+} mk_scan_args;
+MK_API int mk_selective_scan_workspace(const mk_scan_args* args, size_t* bytes);
+MK_API int mk_selective_scan(const mk_scan_args* args, void* stream);
+MK_API int mk_selective_scan_grad_workspace(const mk_scan_args* args, size_t* bytes);
+MK_API int mk_selective_scan_grad(const mk_scan_args* args, void* stream);
+
+/* One token per batch entry: next = the state moved on by one step (next may
+ * be state itself), y as above. */
+typedef struct mk_scan_step_args {
+  int32_t type, softplus;
+  int64_t D, N, G, B;
+  const int32_t* slots;
+  int64_t nslots;
+  const void* u;
+  const void* delta;
+  const void* z;
+  const void* Bmat;
+  const void* Cmat;
+  int64_t ldu, lddelta, ldz, ldb, ldc;
+  const float* A;
+  const float* Dskip;
+  const float* bias;
+  const float* state;           /* (N, D, B or nslots) */
+  float* next;
+  void* y;
+  int64_t ldy;
+} mk_scan_step_args;
+MK_API int mk_selective_scan_step(const mk_scan_step_args* args, void* stream);
+
+/* The norms around a block, its gate and its scaled residual in one pass, per
+ * token column of D channels (mean over the D channels):
+ *   n = hw ? h / sqrt(mean(h^2) + eps) * hw : h       (norm behind the block)
+ *   m = gate ? n * act(gate) : n                      (act: silu, or sigmoid)
+ *   rout = r + (scale ? scale * m : m)                (h == NULL: rout = r)
+ *   y = rout / sqrt(mean(rout^2) + eps) * w           (norm before the next)
+ * y may be NULL (no norm behind the residual; w is then NULL), rout may be
+ * NULL or r itself.  r, rout and their gradients have type rtype (Float32 or
+ * `type`), the others `type`; hw, scale, w are Float32.  The norm of y takes
+ * the unrounded rout.
+ * The gradient takes dy and drout (either may be NULL, not both) and writes dr
+ * and, for each of h, gate, hw, scale, w that is given, its gradient; those of
+ * hw, scale and w are summed over the tokens. */
+#define MK_ACT_SILU    0
+#define MK_ACT_SIGMOID 1
+typedef struct mk_norm_args {
+  int32_t type, rtype, act;
+  float eps;
+  int64_t D, T;
+  const void* r;
+  const void* h;
+  const void* gate;
+  const float* hw;
+  const float* scale;
+  const float* w;
+  void* rout;
+  void* y;
+  int64_t ldr, ldh, ldgate, ldrout, ldy;
+  /* gradient */
+  const void* dy;
+  const void* drout;
+  void* dr;                     /* may be drout itself */
+  void* dh;
+  void* dgate;
+  float* dhw;
+  float* dscale;
+  float* dw;
+  int64_t lddy, lddrout, lddr, lddh, lddgate;
+  void* workspace;
+  size_t workspace_bytes;
+} mk_norm_args;
+MK_API int mk_block_norm(const mk_norm_args* args, void* stream);
+MK_API int mk_block_norm_grad_workspace(const mk_norm_args* args, size_t* bytes);
+MK_API int mk_block_norm_grad(const mk_norm_args* args, void* stream);
+
 /* ---- memory pools -------------------------------------------------------
  * Device memory from a per-device stream-ordered pool that keeps freed memory
  * cached (allocation and free are ordered on `stream`); replaces the CUDA.jl

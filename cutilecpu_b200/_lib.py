@@ -23,7 +23,7 @@ MK_OP = {"add": 0, "max": 1, "min": 2, "mul": 3}
 
 MK_T = {"Float32": 0, "Float16": 1, "BFloat16": 2}
 MK_ACT = {"silu": 0, "sigmoid": 1}
-MK_SCAN_PIECE = 64
+MK_SCAN_PIECE = 32
 
 
 # Argument structs of the state space operators, fields as in the header.

@@ -29,6 +29,45 @@ __device__ __forceinline__ void load(float (&f)[V], const T* p) {
   for (int i = 0; i < V; ++i) f[i] = to_f(v.v[i]);
 }
 
+// r = *p where `on`, else r stays.  A predicated load that stays where it is
+// written: as an ordinary conditional load the compiler may move it down to its
+// use, behind the work that it is to overlap with, or join it with the value
+// for !on by a move that waits for it on the spot.
+template <typename X>
+__device__ __forceinline__ void load_if(X& r, const X* p, bool on) {
+  const unsigned q = on;
+  if constexpr (sizeof(X) == 16) {
+    uint4 v;
+    memcpy(&v, &r, 16);
+    asm volatile("{ .reg .pred q; setp.ne.u32 q, %5, 0; @q ld.global.v4.u32 {%0, %1, %2, %3}, [%4]; }"
+                 : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+                 : "l"(p), "r"(q));
+    memcpy(&r, &v, 16);
+  } else if constexpr (sizeof(X) == 8) {
+    uint2 v;
+    memcpy(&v, &r, 8);
+    asm volatile("{ .reg .pred q; setp.ne.u32 q, %3, 0; @q ld.global.v2.u32 {%0, %1}, [%2]; }"
+                 : "+r"(v.x), "+r"(v.y)
+                 : "l"(p), "r"(q));
+    memcpy(&r, &v, 8);
+  } else if constexpr (sizeof(X) == 4) {
+    unsigned v;
+    memcpy(&v, &r, 4);
+    asm volatile("{ .reg .pred q; setp.ne.u32 q, %2, 0; @q ld.global.u32 %0, [%1]; }" : "+r"(v) : "l"(p), "r"(q));
+    memcpy(&r, &v, 4);
+  } else {
+    static_assert(sizeof(X) == 2, "no such vector");
+    unsigned short v;
+    memcpy(&v, &r, 2);
+    asm volatile("{ .reg .pred q; setp.ne.u32 q, %2, 0; @q ld.global.u16 %0, [%1]; }" : "+h"(v) : "l"(p), "r"(q));
+    memcpy(&r, &v, 2);
+  }
+}
+
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+
 template <typename T, int V>
 __device__ __forceinline__ void store(T* p, const float (&f)[V]) {
   Vec<T, V> v;
@@ -110,6 +149,8 @@ __device__ __forceinline__ void check_distinct(const int32_t* slots, int64_t i, 
 }
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2eLow = 1.92596299e-8f;  // log2(e) - kLog2e
+constexpr float kLn2 = 0.69314718055994530942f;
 
 // 2^x by the special function unit (relative error about 2^-22).
 __device__ __forceinline__ float ex2(float x) {
@@ -118,54 +159,138 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + expf(-x)); }
-
-// log(1 + e^x) = max(x, 0) + log1p(e), e = e^-|x| in (0, 1].  log1p(e) =
-// 2 artanh(s), s = e / (2 + e) <= 1/3: eight terms of the series leave less
-// than 2^-26 relative, so small steps (large negative x) keep full precision,
-// which log(1 + e) in 32 bits loses.
-__device__ __forceinline__ float softplus(float x) {
-  const float e = expf(-fabsf(x));
-  const float s = __fdividef(e, 2.0f + e), w = s * s;
-  float p = 1.0f / 15.0f;
-  p = fmaf(p, w, 1.0f / 13.0f);
-  p = fmaf(p, w, 1.0f / 11.0f);
-  p = fmaf(p, w, 1.0f / 9.0f);
-  p = fmaf(p, w, 1.0f / 7.0f);
-  p = fmaf(p, w, 1.0f / 5.0f);
-  p = fmaf(p, w, 1.0f / 3.0f);
-  p = fmaf(p * w, s, s);
-  return fmaf(2.0f, p, fmaxf(x, 0.0f));
+// Two Float32 values in a register pair, and the packed operations on them:
+// one issue slot for two results.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 pack(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 pack(float a) { return pack(a, a); }
+__device__ __forceinline__ void unpack(F2 x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 ex2_2(F2 x) {
+  float a, b;
+  unpack(x, a, b);
+  return pack(ex2(a), ex2(b));
+}
+__device__ __forceinline__ float sum2(F2 x) {
+  float a, b;
+  unpack(x, a, b);
+  return a + b;
 }
 
-// The sums of v[0..7] over the R lanes that differ in r (lane distance
-// STRIDE), scattered: for R <= 8 lane r ends with the sums of values e * R + r
-// (out[e], e < 8 / R); for R > 8 lanes with equal r % 8 all hold value r % 8.
+// Two neighbouring elements as a pair, and back.
+template <typename T> __device__ __forceinline__ F2 to_f2(const T* p) { return pack(to_f(p[0]), to_f(p[1])); }
+__device__ __forceinline__ void from_f2(float* p, F2 x) { unpack(x, p[0], p[1]); }
+__device__ __forceinline__ void from_f2(__half* p, F2 x) {
+  float a, b;
+  unpack(x, a, b);
+  const __half2 h = __floats2half2_rn(a, b);
+  p[0] = h.x, p[1] = h.y;
+}
+__device__ __forceinline__ void from_f2(__nv_bfloat16* p, F2 x) {
+  float a, b;
+  unpack(x, a, b);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  p[0] = h.x, p[1] = h.y;
+}
+
+// e^x for the elementwise functions.  The rounding of x log2(e) costs |x| 2^-24
+// of the result, which is below what 16-bit inputs bring; Float32 inputs get
+// the product's rounding error back (EXACT).
+template <bool EXACT>
+__device__ __forceinline__ float exp_of(float x) {
+  const float t = x * kLog2e;
+  const float e = ex2(t);
+  if constexpr (!EXACT) return e;
+  const float r = fmaf(x, kLog2eLow, fmaf(x, kLog2e, -t));
+  return fabsf(t) < 150.0f ? fmaf(e, r * kLn2, e) : e;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool EXACT = true>
+__device__ __forceinline__ float sigmoid(float x) { return rcp(1.0f + exp_of<EXACT>(-x)); }
+
+// log(1 + e^x) = max(x, 0) + log1p(e), e = e^-|x| in (0, 1].  log1p(e) = e P(e)
+// with P of degree 8 fitted to log1p(e) / e on [0, 1] for the least relative
+// error (Remez exchange in 64 bits; 3e-8), so small steps (large negative x)
+// keep full precision, which log(1 + e) in 32 bits loses.  With GRAD also the
+// derivative 1 / (1 + e^-x), from the same e.
+__device__ __forceinline__ constexpr float log1p_term(int i) {
+  constexpr float c[9] = {9.999999404e-01f, -4.999949336e-01f, 3.331909776e-01f, -2.484298199e-01f,
+                          1.910600662e-01f, -1.366324574e-01f, 7.822595537e-02f, -2.950523980e-02f,
+                          5.232694093e-03f};
+  return c[i];
+}
+template <bool EXACT = true>
+__device__ __forceinline__ float softplus(float x) {
+  const float e = exp_of<EXACT>(-fabsf(x));
+  float p = log1p_term(8);
+#pragma unroll
+  for (int i = 7; i >= 0; --i) p = fmaf(p, e, log1p_term(i));
+  return fmaf(p, e, fmaxf(x, 0.0f)) + (x != x ? x : 0.0f);
+}
+template <bool EXACT, bool GRAD = false>
+__device__ __forceinline__ F2 softplus2(F2 x, F2* grad = nullptr) {
+  float a, b;
+  unpack(x, a, b);
+  const float ea = exp_of<EXACT>(-fabsf(a)), eb = exp_of<EXACT>(-fabsf(b));
+  const F2 e = pack(ea, eb);
+  F2 p = pack(log1p_term(8));
+#pragma unroll
+  for (int i = 7; i >= 0; --i) p = fma2(p, e, pack(log1p_term(i)));
+  if constexpr (GRAD) {
+    const float ra = rcp(1.0f + ea), rb = rcp(1.0f + eb);
+    *grad = pack(a < 0.0f ? ea * ra : ra, b < 0.0f ? eb * rb : rb);
+  }
+  return fma2(p, e, pack(fmaxf(a, 0.0f), fmaxf(b, 0.0f)));
+}
+
+// The sums of v[0 .. K) over the R <= K lanes that differ in r (lane distance
+// STRIDE), scattered: lane r ends with the sums of values e * R + r (out[e]).
 // Each stage sends half of what is left, so 8 sums over 8 lanes take 7
 // shuffles instead of 24.  The order of the additions is fixed.
-template <int R, int STRIDE>
-__device__ __forceinline__ void reduce_scatter8(float (&v)[8], int r, float (&out)[R < 8 ? 8 / R : 1]) {
-  constexpr int W = R < 8 ? R : 8;
-  constexpr int E = 8 / W;
+template <int K, int R, int STRIDE>
+__device__ __forceinline__ void reduce_scatter(float (&v)[K], int r, float (&out)[K / R]) {
+  constexpr int E = K / R;
 #pragma unroll
-  for (int bit = W / 2; bit >= 1; bit /= 2) {
+  for (int bit = R / 2; bit >= 1; bit /= 2) {
     const bool up = (r & bit) != 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
 #pragma unroll
       for (int q = 0; q < bit; ++q) {
-        const float lo = v[e * W + q], hi = v[e * W + bit + q];
+        const float lo = v[e * R + q], hi = v[e * R + bit + q];
         const float keep = up ? hi : lo, send = up ? lo : hi;
-        v[e * W + q] = keep + __shfl_xor_sync(0xffffffffu, send, bit * STRIDE);
+        v[e * R + q] = keep + __shfl_xor_sync(0xffffffffu, send, bit * STRIDE);
       }
     }
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-#pragma unroll
-    for (int bit = 8; bit < R; bit *= 2) v[e * W] += __shfl_xor_sync(0xffffffffu, v[e * W], bit * STRIDE);
-    out[e] = v[e * W];
-  }
+  for (int e = 0; e < E; ++e) out[e] = v[e * R];
 }
 
 // Runs a C entry point's body: no C++ exception leaves it.

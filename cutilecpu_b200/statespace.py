@@ -232,7 +232,7 @@ def _saved_length(u, A, T: int, nseq: int) -> int:
 
 def selective_scan_saved(u, A, *, seqs=None) -> MLIRArray:
     """An array for the states that ``selective_scan`` leaves for its gradient: one
-    per 64 tokens of a sequence, N floats per channel."""
+    per 32 tokens of a sequence, N floats per channel."""
     c = _Call("selective_scan_saved")
     T, nseq, _, _ = c.sequences(u, seqs)
     with on_device(u, A):

@@ -399,7 +399,7 @@ MK_API int mk_causal_conv_step(const mk_conv_step_args* args, void* stream);
  * The gradient takes dy and, optionally, dlast, and writes du, ddelta, dB, dC,
  * dA, and those of the other inputs that are given (dz, dDskip, dbias: not
  * NULL exactly when z, Dskip, bias are; dinit optional). */
-#define MK_SCAN_PIECE 64
+#define MK_SCAN_PIECE 32
 typedef struct mk_scan_args {
   int32_t type;                 /* MK_T_* of u, delta, z, B, C, y and their gradients */
   int32_t softplus;

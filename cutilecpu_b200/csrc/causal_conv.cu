@@ -5,10 +5,10 @@
 // where x before a sequence's first token is its state (or zero).
 //
 // Bound by memory: 2 reads or writes of the matrix forward, 3 backward, about
-// 4W operations per element.  So a thread owns V neighbouring channels (one
-// 16-byte access forward), keeps their last W - 1 inputs in registers and
-// walks TT tokens; a warp's accesses are one 512-byte row.  The W - 1 tokens
-// before a tile are read again (they hit L2), which is all that is read twice.
+// 4W operations per element.  So a thread owns V neighbouring channels, keeps
+// their last W - 1 inputs in registers and walks TT tokens, with the next
+// tokens' loads in flight while it computes.  The W - 1 tokens before a tile are
+// read again (they hit L2), which is all that is read twice.
 #include "tokens.cuh"
 
 namespace {
@@ -72,18 +72,6 @@ __global__ void __launch_bounds__(kLanes* kRows) conv_last(Conv<T> p) {
   if (d < p.D && s < p.q.nseq) write_last<T, V, W>(p, d, s);
 }
 
-// The last sequence that begins at or before column t.
-__device__ __forceinline__ int64_t seq_at(const Seqs& q, int64_t t) {
-  if (!q.seqs) return q.len ? (t / q.len < q.nseq ? t / q.len : q.nseq - 1) : q.nseq - 1;
-  int64_t lo = 0, hi = q.nseq - 1;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) >> 1;
-    if (seq_offset(q, mid) <= t) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
-
 // One block of a launch looks the offsets and slots over.
 template <typename T>
 __device__ __forceinline__ void check_inputs(const Conv<T>& p, int64_t block, int64_t blocks, int tid, int nt) {
@@ -93,13 +81,54 @@ __device__ __forceinline__ void check_inputs(const Conv<T>& p, int64_t block, in
   }
 }
 
+// A thread's tokens of one matrix, kBatch at a time: kBatches - 1 batches are in
+// flight while one is computed.  Vectors go through a ring in shared memory,
+// single elements (which may be too small to copy) through registers.
+constexpr int kBatch = 4;
+
+template <typename T, int V, int kBatches>
+struct Tokens {
+  static constexpr bool kRing = V > 1;
+  static constexpr int kFlight = kRing ? kBatches - 1 : 1;  // batches asked for ahead
+  static constexpr int kSlots = kRing ? kBatch * kBatches * kLanes * kRows : 1;
+  Vec<T, V> now[kBatch], next[kRing ? 1 : kBatch];
+
+  // Asks for the batch at t (tokens below `end`) as batch number n.
+  __device__ __forceinline__ void ask(Vec<T, V>* ring, const T* x, int64_t ld, int64_t t, int64_t end, int n) {
+    const int tid = threadIdx.y * kLanes + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if constexpr (kRing)
+        copy_if<sizeof(Vec<T, V>)>(ring + ((n % kBatches) * kBatch + j) * kLanes * kRows + tid, x + (t + j) * ld,
+                                   t + j < end);
+      else
+        load_if(next[j], reinterpret_cast<const Vec<T, V>*>(x + (t + j) * ld), t + j < end);
+    }
+  }
+  // Batch n, which has arrived, into `now`.
+  __device__ __forceinline__ void take(const Vec<T, V>* ring, int n) {
+    const int tid = threadIdx.y * kLanes + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if constexpr (kRing) now[j] = ring[((n % kBatches) * kBatch + j) * kLanes * kRows + tid];
+      else now[j] = next[j];
+    }
+  }
+};
+
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(kLanes* kRows) conv_fwd(Conv<T> p) {
+  constexpr bool kExact = sizeof(T) == 4;
+  using X = Tokens<T, V, 4>;
+  __shared__ Vec<T, V> ring[X::kSlots];
+  constexpr int kFlight = X::kFlight;
   const int64_t d = ((int64_t)blockIdx.y * kLanes + threadIdx.x) * V;
   const int64_t tile = (int64_t)blockIdx.x * kRows + threadIdx.y;
   if (blockIdx.y == 0) check_inputs(p, blockIdx.x, gridDim.x, threadIdx.y * kLanes + threadIdx.x, kLanes * kRows);
-  if (d >= p.D || tile >= p.tiles) return;
+  if (tile >= p.tiles) return;
   const int64_t t0 = tile * p.tt, t1 = min(p.q.T, t0 + p.tt);
+  const int64_t s0 = seq_at(p.q, t0);
+  if (d >= p.D) return;
   float w[W][V], bias[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -108,39 +137,49 @@ __global__ void __launch_bounds__(kLanes* kRows) conv_fwd(Conv<T> p) {
     bias[i] = p.bias ? p.bias[d + i] : 0.0f;
   }
   int64_t t = t0;
-  const int64_t s0 = seq_at(p.q, t0);
   for (int64_t s = s0; s < p.q.nseq && t < t1; ++s) {
     const Span sp = seq_span(p.q, s);
     if (sp.hi <= t) continue;
     const int64_t a = max(t, sp.lo), b = min(t1, sp.hi);
     if (a >= b) break;
+    X x;
+#pragma unroll
+    for (int n = 0; n < kFlight; ++n) x.ask(ring, p.x + d, p.ldx, a + n * kBatch, b, n), copy_commit();
     const int64_t row = p.init ? slot_of(p.slots, p.nslots, s, p.err) : -1;
-    float seen[W][V];  // the last W - 1 inputs and the present one
+    float seen[W - 1][V];  // the last W - 1 inputs
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) load_seen<T, V, W>(seen[k], p, d, a - (W - 1) + k, sp.lo, row);
-    constexpr int U = 4;  // tokens loaded ahead of their use
-    for (t = a; t < b; t += U) {
-      float in[U][V];
+    int n = 0;
+    for (t = a; t < b; t += kBatch, ++n) {
+      if (X::kRing) {
+        x.ask(ring, p.x + d, p.ldx, t + kFlight * kBatch, b, n + kFlight);
+        copy_commit();
+        copy_wait<kFlight>();
+        x.take(ring, n);
+      } else {
+        x.take(ring, n);
+        x.ask(ring, p.x + d, p.ldx, t + kBatch, b, n + 1);
+      }
 #pragma unroll
-      for (int j = 0; j < U; ++j)
-        if (t + j < b) load<T, V>(in[j], p.x + (t + j) * p.ldx + d);
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
+      for (int j = 0; j < kBatch; ++j) {
         if (t + j >= b) break;
         float out[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          seen[W - 1][i] = in[j][i];
+          const float v = to_f(x.now[j].v[i]);
           float acc = bias[i];
 #pragma unroll
-          for (int k = 0; k < W; ++k) acc = fmaf(w[k][i], seen[k][i], acc);
-          out[i] = p.silu ? acc * sigmoid(acc) : acc;
+          for (int k = 0; k < W - 1; ++k) acc = fmaf(w[k][i], seen[k][i], acc);
+          acc = fmaf(w[W - 1][i], v, acc);
+          out[i] = p.silu ? acc * sigmoid<kExact>(acc) : acc;
 #pragma unroll
-          for (int k = 0; k < W - 1; ++k) seen[k][i] = seen[k + 1][i];
+          for (int k = 0; k < W - 2; ++k) seen[k][i] = seen[k + 1][i];
+          seen[W - 2][i] = v;
         }
         store<T, V>(p.y + (t + j) * p.ldy + d, out);
       }
     }
+    copy_wait<0>();
     t = b;
   }
   if (p.last) {  // states of the sequences that begin in this tile (the last tile: or behind it)
@@ -161,14 +200,19 @@ __global__ void __launch_bounds__(kLanes* kRows) conv_fwd(Conv<T> p) {
 // summed over the tile in registers, over the block's tiles in shared memory,
 // and over blocks by a second launch in a fixed order (no atomics).
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(kLanes* kRows) conv_bwd(Conv<T> p) {
+__global__ void __launch_bounds__(kLanes* kRows, 3) conv_bwd(Conv<T> p) {
+  using X = Tokens<T, V, sizeof(T) == 4 ? 2 : 4>;  // two rings of Float32: as many as 48 KB hold
+  __shared__ Vec<T, V> ring_x[X::kSlots], ring_dy[X::kSlots];
   __shared__ float sm[kRows][(W + 1) * V][kLanes];
+  constexpr int kFlight = X::kFlight;
   const int64_t d = ((int64_t)blockIdx.y * kLanes + threadIdx.x) * V;
   const int64_t tile = (int64_t)blockIdx.x * kRows + threadIdx.y;
   if (blockIdx.y == 0) check_inputs(p, blockIdx.x, gridDim.x, threadIdx.y * kLanes + threadIdx.x, kLanes * kRows);
+  constexpr bool kExact = sizeof(T) == 4;
   float dw[W][V] = {}, db[V] = {};
+  const int64_t t0 = tile * p.tt, t1 = min(p.q.T, t0 + p.tt);
+  const int64_t s0 = tile < p.tiles ? seq_at(p.q, t0) : 0;
   if (d < p.D && tile < p.tiles) {
-    const int64_t t0 = tile * p.tt, t1 = min(p.q.T, t0 + p.tt);
     float w[W][V], bias[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -177,27 +221,37 @@ __global__ void __launch_bounds__(kLanes* kRows) conv_bwd(Conv<T> p) {
       bias[i] = p.bias ? p.bias[d + i] : 0.0f;
     }
     int64_t t = t0;
-    for (int64_t s = seq_at(p.q, t0); s < p.q.nseq && t < t1; ++s) {
+    for (int64_t s = s0; s < p.q.nseq && t < t1; ++s) {
       const Span sp = seq_span(p.q, s);
       if (sp.hi <= t) continue;
       const int64_t a = max(t, sp.lo), b = min(t1, sp.hi);
       if (a >= b) break;
+      const int64_t stop = b + W - 1, end = min(stop, sp.hi);
+      X x, up;
+#pragma unroll
+      for (int n = 0; n < kFlight; ++n) {
+        x.ask(ring_x, p.x + d, p.ldx, a + n * kBatch, end, n);
+        up.ask(ring_dy, p.dy + d, p.lddy, a + n * kBatch, end, n);
+        copy_commit();
+      }
       float seen[W][V], win[W][V] = {};
 #pragma unroll
       for (int k = 0; k < W - 1; ++k) load_seen<T, V, W>(seen[k], p, d, a - (W - 1) + k, sp.lo, s);
-      const int64_t stop = b + W - 1;
-      constexpr int U = 4;
-      for (int64_t c = a; c < stop; c += U) {
-        float in[U][V], up[U][V];
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          if (c + j < min(stop, sp.hi)) {
-            load<T, V>(in[j], p.x + (c + j) * p.ldx + d);
-            load<T, V>(up[j], p.dy + (c + j) * p.lddy + d);
-          }
+      int n = 0;
+      for (int64_t c = a; c < stop; c += kBatch, ++n) {
+        if (X::kRing) {
+          x.ask(ring_x, p.x + d, p.ldx, c + kFlight * kBatch, end, n + kFlight);
+          up.ask(ring_dy, p.dy + d, p.lddy, c + kFlight * kBatch, end, n + kFlight);
+          copy_commit();
+          copy_wait<kFlight>();
+          x.take(ring_x, n), up.take(ring_dy, n);
+        } else {
+          x.take(ring_x, n), up.take(ring_dy, n);
+          x.ask(ring_x, p.x + d, p.ldx, c + kBatch, end, n + 1);
+          up.ask(ring_dy, p.dy + d, p.lddy, c + kBatch, end, n + 1);
         }
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
+        for (int j = 0; j < kBatch; ++j) {
           const int64_t at = c + j;
           if (at >= stop) break;
           const bool inside = at < sp.hi;
@@ -206,13 +260,13 @@ __global__ void __launch_bounds__(kLanes* kRows) conv_bwd(Conv<T> p) {
           for (int i = 0; i < V; ++i) {
             float dp = 0.0f;
             if (inside) {
-              seen[W - 1][i] = in[j][i];
-              dp = up[j][i];
+              seen[W - 1][i] = to_f(x.now[j].v[i]);
+              dp = to_f(up.now[j].v[i]);
               if (p.silu) {
                 float pre = bias[i];
 #pragma unroll
                 for (int k = 0; k < W; ++k) pre = fmaf(w[k][i], seen[k][i], pre);
-                const float sg = sigmoid(pre);
+                const float sg = sigmoid<kExact>(pre);
                 dp *= sg * fmaf(pre, 1.0f - sg, 1.0f);
               }
               if (at < b) {
@@ -242,6 +296,7 @@ __global__ void __launch_bounds__(kLanes* kRows) conv_bwd(Conv<T> p) {
           else if (a == sp.lo && p.dinit) store<T, V>(p.dinit + (s * (W - 1) + (o - sp.lo + W - 1)) * p.D + d, out);
         }
       }
+      copy_wait<0>();
       t = b;
     }
   }
@@ -312,7 +367,7 @@ __global__ void __launch_bounds__(128) conv_step(ConvStep<T> p) {
     float acc = p.bias ? p.bias[d + i] : 0.0f;
 #pragma unroll
     for (int k = 0; k < W; ++k) acc = fmaf(p.w[k * p.D + d + i], seen[k][i], acc);
-    out[i] = p.silu ? acc * sigmoid(acc) : acc;
+    out[i] = p.silu ? acc * sigmoid<sizeof(T) == 4>(acc) : acc;
   }
 #pragma unroll
   for (int k = 0; k < W - 1; ++k) store<T, V>(p.next + (row * (W - 1) + k) * p.D + d, seen[k + 1]);
@@ -375,7 +430,7 @@ template <typename T, int V, int W>
 int run_fwd(const mk_conv_args* a, mk::Device* dev, cudaStream_t s) {
   Conv<T> p = params<T>(a, dev);
   const int64_t dblocks = mk::cdiv(a->D, kLanes * V);
-  p.tt = tokens_per_tile(dev, a->T, dblocks, 32);
+  p.tt = tokens_per_tile(dev, a->T, dblocks, 64);
   p.tiles = a->T ? mk::cdiv(a->T, p.tt) : 1;
   // A tile may still read the state that another tile's sequence is about to
   // replace: pools that share memory are written by a launch of their own.
@@ -400,7 +455,7 @@ struct BwdPlan {
 BwdPlan plan_bwd(const mk_conv_args* a, const mk::Device* dev) {
   const size_t es = type_bytes(a->type);
   BwdPlan b;
-  const int V = 4;  // 8 of the 16-bit types would not fit the registers
+  const int V = 4;
   const bool vec = a->D % V == 0 && vec_ok(a->x, a->ldx, es, V) && vec_ok(a->dy, a->lddy, es, V) &&
                    vec_ok(a->dx, a->lddx, es, V) && vec_ok(a->init, 0, es, V) && vec_ok(a->dinit, 0, es, V) &&
                    vec_ok(a->dlast, 0, es, V);
@@ -451,12 +506,13 @@ int by_width(int width, F&& f) {
   }
 }
 
-// V2: elements per access of the 16-bit types (Float32: 4).
-template <int V2, typename F>
+// A thread takes four channels, or one where alignment does not allow it.  (Eight of a 16-bit type would be one
+// 16-byte access, but their taps and history leave fewer threads and fewer bytes in flight.)
+template <typename F>
 int dispatch(int type, int width, bool vec, F&& f) {
   if (type == MK_T_F32) return vec ? by_width<float, 4>(width, f) : by_width<float, 1>(width, f);
-  if (type == MK_T_F16) return vec ? by_width<__half, V2>(width, f) : by_width<__half, 1>(width, f);
-  return vec ? by_width<__nv_bfloat16, V2>(width, f) : by_width<__nv_bfloat16, 1>(width, f);
+  if (type == MK_T_F16) return vec ? by_width<__half, 4>(width, f) : by_width<__half, 1>(width, f);
+  return vec ? by_width<__nv_bfloat16, 4>(width, f) : by_width<__nv_bfloat16, 1>(width, f);
 }
 
 struct FwdOp {
@@ -493,10 +549,10 @@ int forward(const mk_conv_args* a, void* stream) {
   if (a->y == a->x && a->T) return bad(who, "y must not be x (later tokens read it)");
   if (a->nseq == 0) return MK_OK;
   MK_ENTRY_DEVICE(dev);
-  const int V = es == 2 ? 8 : 4;
+  const int V = 4;
   const bool vec = a->D % V == 0 && vec_ok(a->x, a->ldx, es, V) && vec_ok(a->y, a->ldy, es, V) &&
                    vec_ok(a->init, 0, es, V) && vec_ok(a->last, 0, es, V);
-  return dispatch<8>(a->type, a->width, vec, FwdOp{a, dev, mk::as_stream(stream)});
+  return dispatch(a->type, a->width, vec, FwdOp{a, dev, mk::as_stream(stream)});
 }
 
 int grad_workspace(const mk_conv_args* a, size_t* bytes) {
@@ -529,7 +585,7 @@ int gradient(const mk_conv_args* a, void* stream) {
   const size_t need = (size_t)b.parts * (a->width + 1) * a->D * sizeof(float);
   if (need && (!a->workspace || a->workspace_bytes < need || !elem_aligned(a->workspace, 4)))
     return bad(who, "a workspace of " + std::to_string(need) + " bytes is needed");
-  return dispatch<4>(a->type, a->width, b.V > 1, BwdOp{a, dev, mk::as_stream(stream), b});
+  return dispatch(a->type, a->width, b.V > 1, BwdOp{a, dev, mk::as_stream(stream), b});
 }
 
 int step(const mk_conv_step_args* a, void* stream) {
@@ -550,7 +606,7 @@ int step(const mk_conv_step_args* a, void* stream) {
   const int V = 4;
   const bool vec = a->D % V == 0 && vec_ok(a->x, a->ldx, es, V) && vec_ok(a->y, a->ldy, es, V) &&
                    vec_ok(a->state, 0, es, V) && vec_ok(a->next, 0, es, V);
-  return dispatch<4>(a->type, a->width, vec, StepOp{a, dev, mk::as_stream(stream)});
+  return dispatch(a->type, a->width, vec, StepOp{a, dev, mk::as_stream(stream)});
 }
 
 }  // namespace

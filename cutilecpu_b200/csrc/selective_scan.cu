@@ -8,10 +8,12 @@ using namespace mk::tok;
 using namespace mk::scan;
 
 // One token per batch entry.  Bound by the state: read and written once, 16
-// bytes per lane, P lanes per channel in memory order.
+// bytes per lane and channel, P lanes per channel in memory order.  A thread
+// takes IT channels, so that as many states are in flight and one read of B
+// and C serves them all.
 template <typename T>
 struct Step {
-  int64_t D, N, G, Dg, B, nslots, dblocks;
+  int64_t D, N, G, Dg, B, nslots, tiles, tpg;  // channel tiles, and of one group
   const T *u, *delta, *z, *Bm, *Cm;
   int64_t ldu, lddelta, ldz, ldb, ldc, ldy;
   const float *A, *Dskip, *bias, *state;
@@ -42,43 +44,55 @@ __device__ __forceinline__ void store4(float* at, const float (&h)[4], int64_t n
   }
 }
 
-template <typename T, int P>
+template <typename T, int P, int IT>
 __global__ void __launch_bounds__(128) scan_step(Step<T> p) {
-  const int64_t e = blockIdx.x / p.dblocks, block = blockIdx.x % p.dblocks;
-  if (block == 0) check_distinct(p.slots, e, threadIdx.x, 128, p.err);
+  constexpr bool kExact = sizeof(T) == 4;
+  constexpr int kChannels = 128 / P;  // a block's channels at a time
+  const int64_t e = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
+  const int64_t g = tile / p.tpg, first = tile % p.tpg * (kChannels * IT) + threadIdx.x / P;
+  const int64_t n0 = threadIdx.x % P * 4;
+  if (tile == 0) check_distinct(p.slots, e, threadIdx.x, 128, p.err);
   const int64_t row = slot_of(p.slots, p.nslots, e, p.err);
   if (row < 0) return;
-  const int64_t dc = block * (128 / P) + threadIdx.x / P, n0 = threadIdx.x % P * 4;
-  const bool live = dc < p.D;
-  const int64_t d = live ? dc : 0, g = d / p.Dg, at = (row * p.D + d) * p.N;
-  float h[4], A[4], b[4], c[4];
-  load4(h, p.state + at, n0, p.N);
-  load4(A, p.A + d * p.N, n0, p.N);
+  float h[IT][4], A[IT][4], b[4], c[4], dt[IT], u[IT], z[IT];
+  int64_t d[IT];
+  bool live[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    live[i] = first + i * kChannels < p.Dg;
+    d[i] = g * p.Dg + (live[i] ? first + i * kChannels : 0);
+    load4(h[i], p.state + (row * p.D + d[i]) * p.N, n0, p.N);
+  }
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    load4(A[i], p.A + d[i] * p.N, n0, p.N);
+    u[i] = to_f(p.u[e * p.ldu + d[i]]);
+    dt[i] = to_f(p.delta[e * p.lddelta + d[i]]) + (p.bias ? p.bias[d[i]] : 0.0f);
+    z[i] = p.z ? to_f(p.z[e * p.ldz + d[i]]) : 0.0f;
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     b[j] = n0 + j < p.N ? to_f(p.Bm[e * p.ldb + g * p.N + n0 + j]) : 0.0f;
     c[j] = n0 + j < p.N ? to_f(p.Cm[e * p.ldc + g * p.N + n0 + j]) : 0.0f;
   }
-  const float u = to_f(p.u[e * p.ldu + d]);
-  const float x = to_f(p.delta[e * p.lddelta + d]) + (p.bias ? p.bias[d] : 0.0f);
-  const float dt = p.softplus ? softplus(x) : x;
-  float y = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    h[j] = fmaf(ex2(dt * (A[j] * kLog2e)), h[j], dt * u * b[j]);
-    y = fmaf(c[j], h[j], y);
-  }
+  for (int i = 0; i < IT; ++i) {
+    if (p.softplus) dt[i] = softplus<kExact>(dt[i]);
+    float y = 0.0f;
 #pragma unroll
-  for (int bit = 1; bit < P; bit *= 2) y += __shfl_xor_sync(0xffffffffu, y, bit);
-  if (!live) return;
-  store4(p.next + at, h, n0, p.N);
-  if (n0 == 0) {
-    y = fmaf(p.Dskip ? p.Dskip[d] : 0.0f, u, y);
-    if (p.z) {
-      const float z = to_f(p.z[e * p.ldz + d]);
-      y *= z * sigmoid(z);
+    for (int j = 0; j < 4; ++j) {
+      h[i][j] = fmaf(decay(dt[i], A[i][j] * kLog2e), h[i][j], dt[i] * u[i] * b[j]);
+      y = fmaf(c[j], h[i][j], y);
     }
-    p.y[e * p.ldy + d] = from_f<T>(y);
+#pragma unroll
+    for (int bit = 1; bit < P; bit *= 2) y += __shfl_xor_sync(0xffffffffu, y, bit);
+    if (!live[i]) continue;
+    store4(p.next + (row * p.D + d[i]) * p.N, h[i], n0, p.N);
+    if (n0 == 0) {
+      y = fmaf(p.Dskip ? p.Dskip[d[i]] : 0.0f, u[i], y);
+      if (p.z) y *= z[i] * sigmoid<kExact>(z[i]);
+      p.y[e * p.ldy + d[i]] = from_f<T>(y);
+    }
   }
 }
 
@@ -194,12 +208,23 @@ int workspace(const char* who, const mk_scan_args* a, bool grad, size_t* bytes) 
   return MK_OK;
 }
 
+template <typename T, int P>
+int launch_step(Step<T> p, const mk::Device* dev, cudaStream_t s) {
+  // four channels per thread, one where that would leave SMs without a block
+  const int64_t four = p.G * mk::cdiv(p.Dg, 4 * (128 / P));
+  const bool wide = four * p.B >= 2 * (int64_t)dev->sms;
+  p.tpg = wide ? four / p.G : mk::cdiv(p.Dg, 128 / P);
+  p.tiles = p.G * p.tpg;
+  const unsigned grid = (unsigned)(p.B * p.tiles);
+  if (wide) scan_step<T, P, 4><<<grid, 128, 0, s>>>(p);
+  else scan_step<T, P, 1><<<grid, 128, 0, s>>>(p);
+  return mk::check_launch("mk_selective_scan_step: launch");
+}
+
 template <typename T>
 int run_step(const mk_scan_step_args* a, const mk::Device* dev, cudaStream_t s) {
   Step<T> p{};
-  const int P = a->N <= 4 ? 1 : a->N <= 8 ? 2 : a->N <= 16 ? 4 : a->N <= 32 ? 8 : 16;
   p.D = a->D, p.N = a->N, p.G = a->G, p.Dg = a->D / a->G, p.B = a->B, p.nslots = a->nslots;
-  p.dblocks = mk::cdiv(a->D, 128 / P);
   p.u = static_cast<const T*>(a->u), p.ldu = a->ldu;
   p.delta = static_cast<const T*>(a->delta), p.lddelta = a->lddelta;
   p.z = static_cast<const T*>(a->z), p.ldz = a->ldz;
@@ -208,15 +233,10 @@ int run_step(const mk_scan_step_args* a, const mk::Device* dev, cudaStream_t s) 
   p.y = static_cast<T*>(a->y), p.ldy = a->ldy;
   p.A = a->A, p.Dskip = a->Dskip, p.bias = a->bias, p.state = a->state, p.next = a->next;
   p.slots = a->slots, p.softplus = a->softplus, p.err = dev->err_word;
-  const unsigned grid = (unsigned)(a->B * p.dblocks);
-  switch (P) {
-    case 1: scan_step<T, 1><<<grid, 128, 0, s>>>(p); break;
-    case 2: scan_step<T, 2><<<grid, 128, 0, s>>>(p); break;
-    case 4: scan_step<T, 4><<<grid, 128, 0, s>>>(p); break;
-    case 8: scan_step<T, 8><<<grid, 128, 0, s>>>(p); break;
-    default: scan_step<T, 16><<<grid, 128, 0, s>>>(p); break;
-  }
-  return mk::check_launch("mk_selective_scan_step: launch");
+  if (a->N <= 4) return launch_step<T, 1>(p, dev, s);
+  if (a->N <= 8) return launch_step<T, 2>(p, dev, s);
+  if (a->N <= 16) return launch_step<T, 4>(p, dev, s);
+  return a->N <= 32 ? launch_step<T, 8>(p, dev, s) : launch_step<T, 16>(p, dev, s);
 }
 
 int step(const mk_scan_step_args* a, void* stream) {
@@ -238,7 +258,7 @@ int step(const mk_scan_step_args* a, void* stream) {
   MK_TRY(check_floats(who, "next", a->next, some, vec));
   if (a->slots && a->nslots < 0) return bad(who, "negative number of slots");
   if (!some) return MK_OK;
-  if (a->B * mk::cdiv(a->D, 8) > INT32_MAX) return bad(who, "batch too large for these channels");
+  if (a->B * (mk::cdiv(a->D, 8) + a->G) > INT32_MAX) return bad(who, "batch too large for these channels");
   MK_ENTRY_DEVICE(dev);
   cudaStream_t s = mk::as_stream(stream);
   if (a->type == MK_T_F32) return run_step<float>(a, dev, s);

@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
         load_states<NS>(add, ws + (k + 1) * p.D * p.N, n0, p.N);
         const F2 sum = pack(wd[k * p.D], wd[k * p.D]);
 #pragma unroll
-        for (int j = 0; j < H; ++j) h[i][j] = fma2(ex2_2(mul2(A2[i][j], sum)), h[i][j], add[j]);
+        for (int j = 0; j < H; ++j) h[i][j] = fma2(decay2(sum, A2[i][j]), h[i][j], add[j]);
       }
     }
   }
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
           dtu[k][i] = v.y;
           if (!FULL) sum_dt[i] += v.x;
 #pragma unroll
-          for (int j = 0; j < H; ++j) a[k][i][j] = mul2(pack(v.x, v.x), A2[i][j]);
+          for (int j = 0; j < H; ++j) a[k][i][j] = fma2(pack(v.x), A2[i][j], pack(kDecayBias));
         }
 #pragma unroll
       for (int k = 0; k < K; ++k)
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(kThreads) scan_rev(Scan<T> p) {
           const float2 v = cells[(q * K + k) * CB + at[i][k % KV]];
           const F2 dt = pack(v.x, v.x), dyp = pack(v.y, v.y);
 #pragma unroll
-          for (int j = 0; j < H; ++j) e_[i][j] = mul2(ex2_2(mul2(dt, A2[i][j])), fma2(c[j], dyp, e_[i][j]));
+          for (int j = 0; j < H; ++j) e_[i][j] = mul2(decay2(dt, A2[i][j]), fma2(c[j], dyp, e_[i][j]));
           sum_dt[i] += v.x;
         }
       }
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, NS * CH <= 4 ? 4 : 2) scan_bwd(Scan<
           const float s1 = p.wsum[(it.first + k) * p.D + w.d[i]];
           const F2 sum = pack(s1, s1);
 #pragma unroll
-          for (int j = 0; j < H; ++j) e_[i][j] = fma2(ex2_2(mul2(A2[i][j], sum)), e_[i][j], add[j]);
+          for (int j = 0; j < H; ++j) e_[i][j] = fma2(decay2(sum, A2[i][j]), e_[i][j], add[j]);
         }
       }
     }
@@ -862,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, NS * CH <= 4 ? 4 : 2) scan_bwd(Scan<
             const float2 v = sm.X[(q * K + k) * CB + at[i][k % KV]];
             const F2 dt = pack(v.x, v.x), dtu = pack(v.y, v.y);
 #pragma unroll
-            for (int j = 0; j < H; ++j) h[i][j] = fma2(ex2_2(mul2(dt, A2[i][j])), h[i][j], mul2(dtu, b[j]));
+            for (int j = 0; j < H; ++j) h[i][j] = fma2(decay2(dt, A2[i][j]), h[i][j], mul2(dtu, b[j]));
           }
         }
       }
@@ -888,7 +888,7 @@ __global__ void __launch_bounds__(kThreads, NS * CH <= 4 ? 4 : 2) scan_bwd(Scan<
             F2 acc;
 #pragma unroll
             for (int j = 0; j < H; ++j) {
-              a[k][i][j] = ex2_2(mul2(dt, A2[i][j]));
+              a[k][i][j] = decay2(dt, A2[i][j]);
               hh[k][i][j] = fma2(a[k][i][j], k ? hh[k ? k - 1 : 0][i][j] : h[i][j], mul2(dtu, b[j]));
               acc = j ? fma2(c[j], hh[k][i][j], acc) : mul2(c[j], hh[k][i][j]);
             }

@@ -64,6 +64,33 @@ __device__ __forceinline__ void load_if(X& r, const X* p, bool on) {
   }
 }
 
+// Asynchronous copies into shared memory (4, 8 or 16 bytes): loads that cost no
+// registers while they are in flight.  The users below copy and read back per
+// thread, so they wait for their own groups of copies and need no barrier.
+template <int BYTES>
+__device__ __forceinline__ void copy_if(void* smem, const void* p, bool on) {
+  const unsigned to = (unsigned)__cvta_generic_to_shared(smem), q = on;
+  if constexpr (BYTES == 16) {
+    asm volatile("{ .reg .pred q; setp.ne.u32 q, %2, 0; @q cp.async.cg.shared.global [%0], [%1], 16; }" ::"r"(to),
+                 "l"(p), "r"(q)
+                 : "memory");
+  } else {
+    asm volatile("{ .reg .pred q; setp.ne.u32 q, %2, 0; @q cp.async.ca.shared.global [%0], [%1], %3; }" ::"r"(to),
+                 "l"(p), "r"(q), "n"(BYTES)
+                 : "memory");
+  }
+}
+// 16 bytes, or zeros where not `on` (p is an address that may be read all the same).
+__device__ __forceinline__ void copy_or_zero(void* smem, const void* p, bool on) {
+  const unsigned to = (unsigned)__cvta_generic_to_shared(smem), bytes = on ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(p), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
 __device__ __forceinline__ void prefetch_l2(const void* p) {
   asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
@@ -103,6 +130,25 @@ __device__ __forceinline__ Span seq_span(const Seqs& q, int64_t s) {
   const bool bad = lo < 0 || hi > q.T || hi < lo;
   const int64_t at = lo < 0 ? 0 : (lo > q.T ? q.T : lo);
   return {at, bad ? at : hi, bad};
+}
+
+// The last sequence that begins at or before column t (the first, if none
+// does), found by a whole warp: 32 offsets are looked at in one round.
+__device__ __forceinline__ int64_t seq_at(const Seqs& q, int64_t t) {
+  if (!q.seqs) {
+    const int64_t s = q.len ? t / q.len : q.nseq - 1;
+    return s < q.nseq ? s : q.nseq - 1;
+  }
+  int64_t lo = 0, count = q.nseq;
+  while (count > 1) {
+    const int64_t step = (count + 31) / 32, at = (threadIdx.x & 31) * step;
+    const unsigned hit = __ballot_sync(0xffffffffu, at < count && seq_offset(q, lo + at) <= t);
+    const int c = __popc(hit);
+    const int64_t skip = c ? (c - 1) * step : 0;
+    lo += skip;
+    count = count - skip < step ? count - skip : step;
+  }
+  return lo;
 }
 
 // A sequence cut into pieces of `piece` columns (the last one shorter): piece
@@ -198,6 +244,14 @@ __device__ __forceinline__ float sum2(F2 x) {
   unpack(x, a, b);
   return a + b;
 }
+
+// exp(dt A) with A2 = A log2(e).  ex2.approx errs low by 2e-8 on average for
+// exponents down to -0.25 (measured against 64 bits), and a slow decay adds
+// that up over its memory of hundreds of tokens: the exponent gets it back, in
+// the same instruction.  A step of dt = 0 still gives exactly 1.
+constexpr float kDecayBias = 3.0e-8f;
+__device__ __forceinline__ float decay(float dt, float A2) { return ex2(fmaf(dt, A2, kDecayBias)); }
+__device__ __forceinline__ F2 decay2(F2 dt, F2 A2) { return ex2_2(fma2(dt, A2, pack(kDecayBias))); }
 
 // Two neighbouring elements as a pair, and back.
 template <typename T> __device__ __forceinline__ F2 to_f2(const T* p) { return pack(to_f(p[0]), to_f(p[1])); }

@@ -298,6 +298,23 @@ def current_stream_handle() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def launch(entry, args, arrays, what: str) -> None:
+    """``entry(args, stream)`` on the current stream of the device that holds
+    ``arrays``, which is made current for the call (like ``on_device``, without
+    its context where nothing has to change)."""
+    dev = arrays[0].storage.get_device()
+    for a in arrays:
+        if a.storage.get_device() != dev:
+            on_device(*arrays)  # names the devices
+    if dev == torch._C._cuda_getDevice():
+        rc = entry(args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, what)
+
+
 def synchronize(backend) -> None:
     """``KA.synchronize``: wait for the device, then raise KernelException if a
     kernel flagged bad input (CUDA.jl's exception check, ext/MLIRCUDAExt.jl:317-335)."""

@@ -4,14 +4,12 @@
 //     y = rout / rms(rout) * w,   rms(x) = sqrt(mean(x^2) + eps).
 //
 // Bound by memory: every matrix is read or written once; a column stays in
-// registers between its reductions (V * ITEMS values per thread).  A column
-// of up to 32 * V * ITEMS channels is one warp's (shuffles only), wider ones a
-// block's.  Blocks walk columns: the next ones are on their way into shared
-// memory while one is computed, and mean(h^2), which is needed first, is
-// reduced together with the column before's last sum, so that a column costs
-// one reduction forward and two backward.  Backward recomputes the forward
-// values from r, h and gate, which costs no more reads than saving rout and
-// its rms would.
+// registers between its reductions, as it is in memory.  A column of up to 32 *
+// V * ITEMS channels is one warp's (shuffles only), wider ones a block's.
+// Products are taken in pairs (f32x2): at 8 or 16 values per thread the issue
+// slots are as scarce as the bandwidth.  Backward recomputes the forward values
+// from r, h and gate, which costs no more reads than saving rout and its rms
+// would.
 #include "tokens.cuh"
 
 namespace {
@@ -34,24 +32,29 @@ struct Norm {
 
 // Sums of two values over the blockDim.x threads of a column.  A column is one
 // warp's, or the whole block's: then every thread adds up the warps' sums, and
-// as two buffers alternate one barrier is enough.
+// as buffers take turns one barrier is enough.
+template <int N>  // buffers: sums between two barriers that reuse one
 struct alignas(16) Sums {
-  float2 part[2][32];  // zeros where there is no warp
+  float2 part[N][32];  // zeros where there is no warp
   __device__ __forceinline__ void clear() {
-    const int i = threadIdx.y * blockDim.x + threadIdx.x;
-    if (i < 64) part[i / 32][i % 32] = make_float2(0.0f, 0.0f);
-    if (blockDim.x * blockDim.y < 64 && i < 32) part[1][i] = make_float2(0.0f, 0.0f);
+    for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < N * 32; i += blockDim.x * blockDim.y)
+      part[i / 32][i % 32] = make_float2(0.0f, 0.0f);
     __syncthreads();
   }
 };
-__device__ __forceinline__ float2 column_sum(float2 v, Sums& sm, int& turn) {
+template <int N>
+__device__ __forceinline__ float2 column_sum(float2 v, Sums<N>& sm, int& turn) {
+  // each half of the warp adds up one of the two
+  const bool up = (threadIdx.x & 16) != 0;
+  float one = up ? v.y : v.x;
+  one += __shfl_xor_sync(0xffffffffu, up ? v.x : v.y, 16);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  for (int o = 8; o > 0; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
+  if (blockDim.x == 32) {
+    const float other = __shfl_xor_sync(0xffffffffu, one, 16);
+    return up ? make_float2(other, one) : make_float2(one, other);
   }
-  if (blockDim.x == 32) return v;
-  if ((threadIdx.x & 31) == 0) sm.part[turn][threadIdx.x >> 5] = v;
+  if ((threadIdx.x & 15) == 0) (&sm.part[turn][threadIdx.x >> 5].x)[up] = one;
   __syncthreads();
   const ulonglong2* part = reinterpret_cast<const ulonglong2*>(sm.part[turn]);
   F2 a = pack(0.0f), b = pack(0.0f);
@@ -61,7 +64,7 @@ __device__ __forceinline__ float2 column_sum(float2 v, Sums& sm, int& turn) {
   }
   a = add2(a, b);
   unpack(a, v.x, v.y);
-  turn ^= 1;
+  if (++turn == N) turn = 0;
   return v;
 }
 
@@ -92,41 +95,28 @@ template <typename T, typename R, int V, int ITEMS, bool GRAD>
 struct Column {
   Vec<R, V> r[ITEMS], dro[GRAD ? ITEMS : 1];
   Vec<T, V> h[ITEMS], g[ITEMS], dy[GRAD ? ITEMS : 1];
-  static constexpr int kPR = V * sizeof(R) / 16, kPT = V * sizeof(T) / 16;  // 16-byte pieces of a vector
-  static constexpr int kPieces = ITEMS * (GRAD ? 2 * kPR + 3 * kPT : kPR + 2 * kPT);
 
-  __device__ __forceinline__ void clear() {
+  // Column t; zeros for what is not there.
+  __device__ __forceinline__ void fetch(const Norm<T, R>& p, int64_t t) {
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k)
+    for (int k = 0; k < ITEMS; ++k) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         r[k].v[i] = from_f<R>(0.0f), h[k].v[i] = g[k].v[i] = from_f<T>(0.0f);
-        if (GRAD) dro[k].v[i] = from_f<R>(0.0f), dy[k].v[i] = from_f<T>(0.0f);
+        if constexpr (GRAD) dro[k].v[i] = from_f<R>(0.0f), dy[k].v[i] = from_f<T>(0.0f);
       }
-  }
-  // F(vector in registers, its place in memory, whether it is there) for h of column t, and for the rest of it
-  template <typename F>
-  __device__ __forceinline__ void each_h(Vec<T, V> (&h)[ITEMS], const Norm<T, R>& p, int64_t t, F&& f) {
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-      const int64_t d = ((int64_t)k * blockDim.x + threadIdx.x) * V;
-      f(h[k], p.h + t * p.ldh + d, d < p.D && t < p.T_ && p.h);
-    }
-  }
-  template <typename F>
-  __device__ __forceinline__ void each_other(const Norm<T, R>& p, int64_t t, F&& f) {
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
       const int64_t d = ((int64_t)k * blockDim.x + threadIdx.x) * V;
       const bool on = d < p.D && t < p.T_;
-      f(r[k], p.r + t * p.ldr + d, on);
-      f(g[k], p.gate + t * p.ldgate + d, on && p.gate);
+      load_vec<T, V>(h[k], p.h + t * p.ldh + d, on && p.h);
+      load_vec<R, V>(r[k], p.r + t * p.ldr + d, on);
+      load_vec<T, V>(g[k], p.gate + t * p.ldgate + d, on && p.gate);
       if constexpr (GRAD) {
-        f(dy[k], p.dy + t * p.lddy + d, on && p.dy);
-        f(dro[k], p.drout + t * p.lddrout + d, on && p.drout);
+        load_vec<T, V>(dy[k], p.dy + t * p.lddy + d, on && p.dy);
+        load_vec<R, V>(dro[k], p.drout + t * p.lddrout + d, on && p.drout);
       }
     }
   }
+  __device__ __forceinline__ float sum_hh() const;
 };
 
 // Values 2 j and 2 j + 1 of a thread's vectors, and back.
@@ -153,295 +143,174 @@ __device__ __forceinline__ void store_column(X* column, int64_t D, const Vec<X, 
   }
 }
 
-// The columns that a thread walks, one after another.  S > 1: S - 1 of them are
-// on their way into shared memory while one is computed; every thread copies
-// and reads back its own 16-byte pieces, so no barrier is needed.  S == 1:
-// straight from memory.
-template <typename T, typename R, int V, int ITEMS, bool GRAD, int S>
-struct Walk {
-  using C = Column<T, R, V, ITEMS, GRAD>;
-  C now;
-  Vec<T, V> h_next[ITEMS];
-  uint4* stages;
-  int tid, nt, n = 0;  // n: the stage of the next column
-  int64_t stride;
-
-  __device__ __forceinline__ uint4* piece(int stage, int i) { return stages + (stage * C::kPieces + i) * nt + tid; }
-  __device__ __forceinline__ void copy(const Norm<T, R>& p, int64_t t, int stage) {
-    int i = 0;
-    auto f = [&](auto& r, auto* at, bool on) {
+template <typename T, typename R, int V, int ITEMS, bool GRAD>
+__device__ __forceinline__ float Column<T, R, V, ITEMS, GRAD>::sum_hh() const {
+  F2 s = pack(0.0f);
 #pragma unroll
-      for (int x = 0; x < (int)(sizeof(r) / 16); ++x)
-        copy_or_zero(piece(stage, i++), on ? (const void*)(reinterpret_cast<const uint4*>(at) + x) : p.r, on);
-    };
-    now.each_h(now.h, p, t, f);
-    now.each_other(p, t, f);
-    copy_commit();
+  for (int j = 0; j < V * ITEMS / 2; ++j) {
+    const F2 x = pair_at(h, j);
+    s = fma2(x, x, s);
   }
-  __device__ __forceinline__ Walk(const Norm<T, R>& p, int64_t t, int64_t stride_, uint4* smem) : stride(stride_) {
-    stages = smem;
-    tid = threadIdx.y * blockDim.x + threadIdx.x;
-    nt = blockDim.x * blockDim.y;
-    now.clear();
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) h_next[k] = now.h[k];
-    if constexpr (S > 1) {
-#pragma unroll
-      for (int i = 0; i < S - 1; ++i) copy(p, t + i * stride, i);
-    }
-  }
-  // h of column t, the next one, into h_next.
-  __device__ __forceinline__ void take_h(const Norm<T, R>& p, int64_t t) {
-    if constexpr (S > 1) {
-      copy(p, t + (S - 1) * stride, n == 0 ? S - 1 : n - 1);
-      copy_wait<S - 1>();
-      int i = 0;
-      now.each_h(h_next, p, t, [&](auto& r, auto*, bool) {
-#pragma unroll
-        for (int x = 0; x < (int)(sizeof(r) / 16); ++x) {
-          const uint4 v = *piece(n, i++);
-          memcpy(reinterpret_cast<char*>(&r) + 16 * x, &v, 16);
-        }
-      });
-    } else {
-      now.each_h(h_next, p, t, [](auto& r, auto* at, bool on) { load_vec(r, at, on); });
-    }
-  }
-  // The rest of it, and its h to where it belongs: column t is now the present one.
-  __device__ __forceinline__ void take_rest(const Norm<T, R>& p, int64_t t) {
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) now.h[k] = h_next[k];
-    if constexpr (S > 1) {
-      int i = ITEMS * C::kPT;
-      now.each_other(p, t, [&](auto& r, auto*, bool) {
-#pragma unroll
-        for (int x = 0; x < (int)(sizeof(r) / 16); ++x) {
-          const uint4 v = *piece(n, i++);
-          memcpy(reinterpret_cast<char*>(&r) + 16 * x, &v, 16);
-        }
-      });
-      n = n + 1 == S ? 0 : n + 1;
-    } else {
-      now.each_other(p, t, [](auto& r, auto* at, bool on) { load_vec(r, at, on); });
-    }
-  }
-  __device__ __forceinline__ float sum_h_next() const {
-    F2 s = pack(0.0f);
-#pragma unroll
-    for (int j = 0; j < V * ITEMS / 2; ++j) {
-      const F2 h = pair_at(h_next, j);
-      s = fma2(h, h, s);
-    }
-    return sum2(s);
-  }
-  __device__ __forceinline__ void end() {
-    if constexpr (S > 1) copy_wait<0>();
-  }
-};
-
-// Values 2 j and 2 j + 1 of a thread's channels of a parameter, ones without it.
-template <int V>
-__device__ __forceinline__ F2 param_at(const float* p, int64_t D, int j) {
-  const int64_t d0 = ((int64_t)(2 * j / V) * blockDim.x + threadIdx.x) * V + 2 * j % V;
-  if constexpr (V > 1) {
-    const F2 one = pack(1.0f);
-    return p && d0 < D ? F2{*reinterpret_cast<const unsigned long long*>(p + d0)} : one;
-  } else {
-    const int64_t d1 = d0 + blockDim.x;
-    return pack(p && d0 < D ? p[d0] : 1.0f, p && d1 < D ? p[d1] : 1.0f);
-  }
+  return sum2(s);
 }
 
-// All of a thread's values of a parameter.
+// A thread's values of a parameter, ones without it.
 template <int V, int ITEMS>
 __device__ __forceinline__ void param(F2 (&f)[V * ITEMS / 2], const float* p, int64_t D) {
+  Vec<float, V> r[ITEMS];
 #pragma unroll
-  for (int j = 0; j < V * ITEMS / 2; ++j) f[j] = param_at<V>(p, D, j);
+  for (int k = 0; k < ITEMS; ++k) {
+    const int d = (k * blockDim.x + threadIdx.x) * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[k].v[i] = 1.0f;
+    load_vec<float, V>(r[k], p + d, p && d < D);
+  }
+#pragma unroll
+  for (int j = 0; j < V * ITEMS / 2; ++j) f[j] = pair_at(r, j);
 }
 
-template <typename T, typename R, int V, int ITEMS, int S>
-__global__ void __launch_bounds__(V * ITEMS <= 8 ? 512 : 1024, 1) norm_fwd(Norm<T, R> p) {
+template <typename T, typename R, int V, int ITEMS, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) norm_fwd(Norm<T, R> p) {
   constexpr bool kExact = sizeof(T) == 4;
-  constexpr bool kHold = V * ITEMS <= 8;  // parameters in registers
-  extern __shared__ uint4 norm_smem[];
-  __shared__ Sums sm;
-  int turn = 0;
-  sm.clear();
-  const int64_t stride = (int64_t)gridDim.x * blockDim.y;
-  int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (t >= p.T_) return;
-  Walk<T, R, V, ITEMS, false, S> walk(p, t, stride, norm_smem);
   constexpr int H = V * ITEMS / 2;
-  F2 hw[H], sc[H], w[H];
-  if constexpr (kHold) param<V, ITEMS>(hw, p.hw, p.D), param<V, ITEMS>(sc, p.scale, p.D), param<V, ITEMS>(w, p.w, p.D);
-  const bool norm_h = p.h && p.hw;
-  walk.take_h(p, t);
+  __shared__ Sums<2> sm;
+  int turn = 0;
+  const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  Column<T, R, V, ITEMS, false> cur;
+  cur.fetch(p, t);
+  sm.clear();
+  if (t >= p.T_) return;
   float i1 = 1.0f;
-  if (norm_h) i1 = rsqrtf(fmaf(column_sum(make_float2(walk.sum_h_next(), 0.0f), sm, turn).x, p.inv_d, p.eps));
-  walk.take_rest(p, t);
-  const auto& cur = walk.now;
-  for (;;) {
-    const bool silu = p.act == MK_ACT_SILU;
-    if constexpr (!kHold) param<V, ITEMS>(hw, p.hw, p.D), param<V, ITEMS>(sc, p.scale, p.D);
-    F2 x[H], sum = pack(0.0f);
-    const F2 i1_2 = pack(i1);
+  if (p.h && p.hw) i1 = rsqrtf(fmaf(column_sum(make_float2(cur.sum_hh(), 0.0f), sm, turn).x, p.inv_d, p.eps));
+  const bool silu = p.act == MK_ACT_SILU;
+  F2 x[H], sum = pack(0.0f);
+  const F2 i1_2 = pack(i1);
+  F2 par[H];
+  param<V, ITEMS>(par, p.hw, p.D);
 #pragma unroll
-    for (int j = 0; j < H; ++j) x[j] = mul2(mul2(pair_at(cur.h, j), i1_2), hw[j]);  // zeros without h
-    if (p.gate) {
-#pragma unroll
-      for (int j = 0; j < H; ++j) {
-        const F2 g = pair_at(cur.g, j);
-        x[j] = mul2(x[j], sigmoid2<kExact>(g));
-        if (silu) x[j] = mul2(x[j], g);
-      }
-    }
+  for (int j = 0; j < H; ++j) x[j] = mul2(mul2(pair_at(cur.h, j), i1_2), par[j]);  // zeros without h
+  if (p.gate) {
 #pragma unroll
     for (int j = 0; j < H; ++j) {
-      x[j] = fma2(sc[j], x[j], pair_at(cur.r, j));
-      sum = fma2(x[j], x[j], sum);  // channels beyond D are zeros
+      const F2 g = pair_at(cur.g, j);
+      x[j] = mul2(x[j], sigmoid2<kExact>(g));
+      if (silu) x[j] = mul2(x[j], g);
     }
-    if (p.rout) {
-      Vec<R, V> out[ITEMS];
-#pragma unroll
-      for (int j = 0; j < H; ++j) put_pair(out, j, x[j]);
-      store_column(p.rout + t * p.ldrout, p.D, out);
-    }
-    float2 s = make_float2(sum2(sum), 0.0f);
-    const int64_t next = t + stride;
-    walk.take_h(p, next);
-    if (norm_h) s.y = walk.sum_h_next();
-    if (p.y || norm_h) s = column_sum(s, sm, turn);
-    if (p.y) {
-      const F2 i2 = pack(rsqrtf(fmaf(s.x, p.inv_d, p.eps)));
-      if constexpr (!kHold) param<V, ITEMS>(w, p.w, p.D);
-      Vec<T, V> out[ITEMS];
-#pragma unroll
-      for (int j = 0; j < H; ++j) put_pair(out, j, mul2(w[j], mul2(x[j], i2)));
-      store_column(p.y + t * p.ldy, p.D, out);
-    }
-    t = next;
-    if (t >= p.T_) break;
-    if (norm_h) i1 = rsqrtf(fmaf(s.y, p.inv_d, p.eps));
-    walk.take_rest(p, t);
   }
-  walk.end();
+  param<V, ITEMS>(par, p.scale, p.D);
+#pragma unroll
+  for (int j = 0; j < H; ++j) {
+    x[j] = fma2(par[j], x[j], pair_at(cur.r, j));
+    sum = fma2(x[j], x[j], sum);  // channels beyond D are zeros
+  }
+  if (p.rout) {
+    Vec<R, V> out[ITEMS];
+#pragma unroll
+    for (int j = 0; j < H; ++j) put_pair(out, j, x[j]);
+    store_column(p.rout + t * p.ldrout, p.D, out);
+  }
+  if (p.y) {
+    param<V, ITEMS>(par, p.w, p.D);
+    const float2 s = column_sum(make_float2(sum2(sum), 0.0f), sm, turn);
+    const F2 i2 = pack(rsqrtf(fmaf(s.x, p.inv_d, p.eps)));
+    Vec<T, V> out[ITEMS];
+#pragma unroll
+    for (int j = 0; j < H; ++j) put_pair(out, j, mul2(par[j], mul2(x[j], i2)));
+    store_column(p.y + t * p.ldy, p.D, out);
+  }
 }
 
 // Backward.  With x = rout i2 and dx = dy w:
 //   dro = drout + i2 (dx - x mean(dx x)),  dr = dro,
 //   dm = dro scale, dn = dm act, dgate = dm n act', dv = dn hw,
 //   dh = i1 (dv - v mean(dv v)), v = h i1;
-// dw += dy x, dhw += dn v, dscale += dro m.  A block walks columns, keeps its
-// sums for w, hw and scale in registers (one part per column walker, added up
-// by norm_fold in a fixed order), and keeps the inputs as they are in memory
-// between its three reductions.
-template <typename T, typename R, int V, int ITEMS, int S>
-__global__ void __launch_bounds__(V * ITEMS <= 8 ? 512 : 1024, 1) norm_bwd(Norm<T, R> p) {
+// dw += dy x, dhw += dn v, dscale += dro m.  A block walks columns and keeps its
+// sums for w, hw and scale in shared memory, every thread its own channels'
+// (in registers they would leave one block to an SM, and two overlap each
+// other's waits); they go to one part per column walker, added up by norm_fold
+// in a fixed order.
+template <typename T, typename R, int V, int ITEMS, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) norm_bwd(Norm<T, R> p) {
   constexpr bool kExact = sizeof(T) == 4;
-  extern __shared__ uint4 norm_smem[];
-  __shared__ Sums sm;
+  constexpr int H = V * ITEMS / 2;
+  extern __shared__ float2 acc_smem[];  // [column walker][3][pair of values][thread]
+  __shared__ Sums<3> sm;
   int turn = 0;
   sm.clear();
   const int64_t stride = (int64_t)gridDim.x * blockDim.y;
   const int64_t walker = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  constexpr int H = V * ITEMS / 2;
-  F2 aw[H], ah[H], as[H];
-#pragma unroll
-  for (int j = 0; j < H; ++j) aw[j] = ah[j] = as[j] = pack(0.0f);
-  // the parameters in shared memory behind the stages, ones for those that are not there
-  const float *p_hw = p.hw, *p_scale = p.scale, *p_w = p.w;
-  if constexpr (S > 1) {
-    float* sp = reinterpret_cast<float*>(norm_smem + S * Column<T, R, V, ITEMS, true>::kPieces * blockDim.x * blockDim.y);
-    for (int64_t i = threadIdx.y * blockDim.x + threadIdx.x; i < p.D; i += blockDim.x * blockDim.y) {
-      sp[i] = p.hw ? p.hw[i] : 1.0f;
-      sp[p.D + i] = p.scale ? p.scale[i] : 1.0f;
-      sp[2 * p.D + i] = p.w ? p.w[i] : 1.0f;
-    }
-    __syncthreads();
-    p_hw = sp, p_scale = sp + p.D, p_w = sp + 2 * p.D;
-  }
-  int64_t t = walker;
-  if (t < p.T_) {
-    Walk<T, R, V, ITEMS, true, S> walk(p, t, stride, norm_smem);
-    const bool norm_h = p.h && p.hw;
-    walk.take_h(p, t);
+  float2* acc = acc_smem + threadIdx.y * 3 * H * blockDim.x + threadIdx.x;
+  for (int i = 0; i < 3 * H; ++i) acc[i * blockDim.x] = make_float2(0.0f, 0.0f);
+  auto add = [&](int which, int j, F2 a, F2 b) {  // a b more
+    unsigned long long* at = reinterpret_cast<unsigned long long*>(acc + (which * H + j) * blockDim.x);
+    *at = fma2(a, b, F2{*at}).v;
+  };
+  const bool silu = p.gate && p.act == MK_ACT_SILU;
+  for (int64_t t = walker; t < p.T_; t += stride) {
+    Column<T, R, V, ITEMS, true> cur;
+    cur.fetch(p, t);
     float i1 = 1.0f;
-    if (norm_h) i1 = rsqrtf(fmaf(column_sum(make_float2(walk.sum_h_next(), 0.0f), sm, turn).x, p.inv_d, p.eps));
-    walk.take_rest(p, t);
-    const auto& cur = walk.now;
-    for (;;) {
-      F2 x[H], sig[H];  // sig: of the gate, ones without
-      const bool silu = p.gate && p.act == MK_ACT_SILU;
-      F2 sxx = pack(0.0f), sdx = pack(0.0f);
-      const F2 i1_2 = pack(i1);
+    if (p.h && p.hw) i1 = rsqrtf(fmaf(column_sum(make_float2(cur.sum_hh(), 0.0f), sm, turn).x, p.inv_d, p.eps));
+    const F2 i1_2 = pack(i1);
+    F2 x[H], sig[H];  // sig: of the gate, ones without
+    F2 sxx = pack(0.0f), sdx = pack(0.0f);
+    F2 hw[H], sc[H], w[H];
+    param<V, ITEMS>(hw, p.hw, p.D), param<V, ITEMS>(sc, p.scale, p.D), param<V, ITEMS>(w, p.w, p.D);
 #pragma unroll
-      for (int j = 0; j < H; ++j) sig[j] = p.gate ? sigmoid2<kExact>(pair_at(cur.g, j)) : pack(1.0f);
-#pragma unroll
-      for (int j = 0; j < H; ++j) {  // without h its values are zeros, without dy those
-        F2 m = mul2(mul2(mul2(pair_at(cur.h, j), i1_2), param_at<V>(p_hw, p.D, j)), sig[j]);
-        if (silu) m = mul2(m, pair_at(cur.g, j));
-        x[j] = fma2(param_at<V>(p_scale, p.D, j), m, pair_at(cur.r, j));
-        sxx = fma2(x[j], x[j], sxx);
-        sdx = fma2(mul2(pair_at(cur.dy, j), param_at<V>(p_w, p.D, j)), x[j], sdx);
-      }
-      float i2 = 0.0f, mean = 0.0f;
-      if (p.dy) {
-        const float2 s = column_sum(make_float2(sum2(sxx), sum2(sdx)), sm, turn);
-        i2 = rsqrtf(fmaf(s.x, p.inv_d, p.eps));
-        mean = s.y * i2 * p.inv_d;
-      }
-      const F2 i2_2 = pack(i2), off = pack(-mean * i2);
-      F2 dv[H], sdv = pack(0.0f);
-      {
-        Vec<R, V> out[ITEMS];
-        Vec<T, V> dg[ITEMS];
-#pragma unroll
-        for (int j = 0; j < H; ++j) {
-          const F2 xh = mul2(x[j], i2_2), dy = pair_at(cur.dy, j);
-          aw[j] = fma2(dy, xh, aw[j]);
-          const F2 dro = fma2(xh, off, fma2(mul2(dy, param_at<V>(p_w, p.D, j)), i2_2, pair_at(cur.dro, j)));
-          put_pair(out, j, dro);
-          const F2 hw = param_at<V>(p_hw, p.D, j);
-          const F2 v = mul2(pair_at(cur.h, j), i1_2), n = mul2(v, hw), dm = mul2(dro, param_at<V>(p_scale, p.D, j));
-          const F2 a = silu ? mul2(sig[j], pair_at(cur.g, j)) : sig[j];
-          as[j] = fma2(dro, mul2(n, a), as[j]);
-          const F2 dn = mul2(dm, a);
-          if (p.gate) put_pair(dg, j, mul2(mul2(dm, n), act_grad(a, sig[j], silu)));
-          ah[j] = fma2(dn, v, ah[j]);
-          dv[j] = mul2(dn, hw);
-          sdv = fma2(dv[j], v, sdv);
-        }
-        store_column(p.dr + t * p.lddr, p.D, out);
-        if (p.gate) store_column(p.dgate + t * p.lddgate, p.D, dg);
-      }
-      const int64_t next = t + stride;
-      walk.take_h(p, next);
-      float back = 0.0f, i1_next = 1.0f;
-      if (norm_h) {
-        const float2 s = column_sum(make_float2(sum2(sdv), walk.sum_h_next()), sm, turn);
-        back = s.x * p.inv_d * i1;
-        i1_next = rsqrtf(fmaf(s.y, p.inv_d, p.eps));
-      }
-      if (p.h) {
-        const F2 minus = pack(-back);
-        Vec<T, V> out[ITEMS];
-#pragma unroll
-        for (int j = 0; j < H; ++j) put_pair(out, j, mul2(i1_2, fma2(pair_at(cur.h, j), minus, dv[j])));
-        store_column(p.dh + t * p.lddh, p.D, out);
-      }
-      t = next;
-      if (t >= p.T_) break;
-      i1 = i1_next;
-      walk.take_rest(p, t);
+    for (int j = 0; j < H; ++j) {  // without h its values are zeros, without dy those
+      sig[j] = p.gate ? sigmoid2<kExact>(pair_at(cur.g, j)) : pack(1.0f);
+      F2 m = mul2(mul2(mul2(pair_at(cur.h, j), i1_2), hw[j]), sig[j]);
+      if (silu) m = mul2(m, pair_at(cur.g, j));
+      x[j] = fma2(sc[j], m, pair_at(cur.r, j));
+      sxx = fma2(x[j], x[j], sxx);
+      sdx = fma2(mul2(pair_at(cur.dy, j), w[j]), x[j], sdx);
     }
-    walk.end();
+    float i2 = 0.0f, mean = 0.0f;
+    if (p.dy) {
+      const float2 s = column_sum(make_float2(sum2(sxx), sum2(sdx)), sm, turn);
+      i2 = rsqrtf(fmaf(s.x, p.inv_d, p.eps));
+      mean = s.y * i2 * p.inv_d;
+    }
+    const F2 i2_2 = pack(i2), off = pack(-mean * i2);
+    F2 sdv = pack(0.0f);
+    param<V, ITEMS>(hw, p.hw, p.D), param<V, ITEMS>(sc, p.scale, p.D), param<V, ITEMS>(w, p.w, p.D);
+    {
+      Vec<R, V> out[ITEMS];
+      Vec<T, V> dg[ITEMS];
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        const F2 xh = mul2(x[j], i2_2), dy = pair_at(cur.dy, j);
+        add(0, j, dy, xh);
+        const F2 dro = fma2(xh, off, fma2(mul2(dy, w[j]), i2_2, pair_at(cur.dro, j)));
+        put_pair(out, j, dro);
+        const F2 v = mul2(pair_at(cur.h, j), i1_2), n = mul2(v, hw[j]), dm = mul2(dro, sc[j]);
+        const F2 a = silu ? mul2(sig[j], pair_at(cur.g, j)) : sig[j];
+        add(2, j, dro, mul2(n, a));
+        const F2 dn = mul2(dm, a);
+        if (p.gate) put_pair(dg, j, mul2(mul2(dm, n), act_grad(a, sig[j], silu)));
+        add(1, j, dn, v);
+        x[j] = mul2(dn, hw[j]);  // from here: the gradient of v
+        sdv = fma2(x[j], v, sdv);
+      }
+      store_column(p.dr + t * p.lddr, p.D, out);
+      if (p.gate) store_column(p.dgate + t * p.lddgate, p.D, dg);
+    }
+    if (p.h) {
+      float back = 0.0f;
+      if (p.hw) back = column_sum(make_float2(sum2(sdv), 0.0f), sm, turn).x * p.inv_d * i1;
+      const F2 minus = pack(-back);
+      Vec<T, V> out[ITEMS];
+#pragma unroll
+      for (int j = 0; j < H; ++j) put_pair(out, j, mul2(i1_2, fma2(pair_at(cur.h, j), minus, x[j])));
+      store_column(p.dh + t * p.lddh, p.D, out);
+    }
   }
   float* part = p.parts + walker * 3 * p.D;
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
     Vec<float, V> out[ITEMS];
 #pragma unroll
-    for (int j = 0; j < H; ++j) put_pair(out, j, i == 0 ? aw[j] : i == 1 ? ah[j] : as[j]);
+    for (int j = 0; j < H; ++j) put_pair(out, j, F2{*reinterpret_cast<unsigned long long*>(acc + (i * H + j) * blockDim.x)});
     store_column(part + i * p.D, p.D, out);
   }
 }
@@ -469,7 +338,7 @@ __global__ void __launch_bounds__(256) norm_fold(const float* parts, int64_t npa
 
 // ---- host side ----------------------------------------------------------------
 
-constexpr int64_t kMostChannels = 16384;
+constexpr int64_t kMostChannels = 16384;  // 16 values for each of 1024 threads
 
 int check(const char* who, const mk_norm_args* a, bool grad) {
   if (!a) return bad(who, "null arguments");
@@ -547,38 +416,24 @@ Norm<T, R> params(const mk_norm_args* a) {
   return p;
 }
 
-// S stages of the column walk in shared memory, and `more` bytes behind them.
-template <int S, typename K, typename... A>
-int launch(K kernel, int64_t grid, dim3 block, int pieces, size_t more, cudaStream_t s, const char* who, A... args) {
-  const size_t smem = S > 1 ? (size_t)S * pieces * 16 * block.x * block.y + more : 0;
-  if (smem) MK_TRY(mk::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem));
-  kernel<<<(unsigned)grid, block, smem, s>>>(args...);
-  return mk::check_launch(who);
-}
-
-template <typename T, typename R, int V, int ITEMS, int S>
-int launch_fwd(const mk_norm_args* a, const mk::Device* dev, cudaStream_t s) {
+template <typename T, typename R, int V, int ITEMS, int THREADS, int BLOCKS>
+int launch_fwd(const mk_norm_args* a, cudaStream_t s) {
   const dim3 block = block_of(a->D, V, ITEMS);
-  int64_t grid = mk::cdiv(a->T, block.y);
-  const int64_t most = (int64_t)dev->sms * (block.x * block.y < 512 ? 512 / (block.x * block.y) : 1);  // resident at once
-  if (grid > most) grid = most;
-  return launch<S>(norm_fwd<T, R, V, ITEMS, S>, grid, block, Column<T, R, V, ITEMS, false>::kPieces, 0, s,
-                   "mk_block_norm: launch", params<T, R>(a));
+  norm_fwd<T, R, V, ITEMS, THREADS, BLOCKS><<<(unsigned)mk::cdiv(a->T, block.y), block, 0, s>>>(params<T, R>(a));
+  return mk::check_launch("mk_block_norm: launch");
 }
 
-// Vectors per thread: as few as keep a column within the block's threads.  Up
-// to 4096 channels the stages fit an SM's shared memory.
+// 16 values per thread; columns of up to 4096 channels take 256 threads at
+// most, so that the registers hold four of them on an SM.
 template <typename T, typename R>
-int run_fwd(const mk_norm_args* a, const mk::Device* dev, cudaStream_t s) {
+int run_fwd(const mk_norm_args* a, cudaStream_t s) {
   constexpr int V = sizeof(T) == 2 ? 8 : 4;
-  if (all_vec(a, V, false)) {
-    if (a->D <= 4096) return launch_fwd<T, R, V, 8 / V, sizeof(T) == 2 ? 3 : 2>(a, dev, s);
-    return launch_fwd<T, R, V, 16 / V, 1>(a, dev, s);
-  }
-  return a->D <= 2048 ? launch_fwd<T, R, 1, 4, 1>(a, dev, s) : launch_fwd<T, R, 1, 16, 1>(a, dev, s);
+  if (all_vec(a, V, false))
+    return a->D <= 4096 ? launch_fwd<T, R, V, 16 / V, 256, 4>(a, s) : launch_fwd<T, R, V, 16 / V, 1024, 1>(a, s);
+  return a->D <= 4096 ? launch_fwd<T, R, 1, 16, 256, 3>(a, s) : launch_fwd<T, R, 1, 16, 1024, 1>(a, s);
 }
 
-// ITEMS vectors of V channels per thread.
+// Values per thread: 8, and 16 of the widest columns.
 struct BwdPlan {
   int V, items;
   dim3 block;
@@ -587,52 +442,48 @@ struct BwdPlan {
 
 BwdPlan plan_bwd(const mk_norm_args* a, const mk::Device* dev) {
   BwdPlan b;
-  const int wide = type_bytes(a->type) == 2 ? 8 : 4;
-  b.V = all_vec(a, wide, true) ? wide : 1;
-  const int64_t n = mk::cdiv(a->D, b.V);
-  if (b.V == 8) b.items = n <= 512 ? 1 : 2;
-  else if (b.V == 4) b.items = n <= 1024 ? 2 : 4;
-  else b.items = n <= 2048 ? 4 : 16;
+  const bool half = type_bytes(a->type) == 2;
+  b.V = all_vec(a, half ? 8 : 4, true) ? (half ? 8 : 4) : 1;
+  b.items = (a->D > 4096 ? 16 : 8) / b.V;
   b.block = block_of(a->D, b.V, b.items);
   const int64_t columns = mk::cdiv(a->T, b.block.y);
   const int64_t threads = (int64_t)b.block.x * b.block.y;
-  const int64_t most = (int64_t)dev->sms * (threads < 512 ? 512 / threads : 1);
+  const int64_t most = (int64_t)dev->sms * (threads < 512 ? 512 / threads : 1);  // resident at once
   b.grid = columns < most ? columns : most;
   b.parts = b.grid * b.block.y;
   return b;
 }
 
-template <typename T, typename R, int V, int ITEMS, int S>
+template <typename T, typename R, int V, int ITEMS, int THREADS, int BLOCKS>
 int launch_bwd(const mk_norm_args* a, const BwdPlan& b, cudaStream_t s) {
   const Norm<T, R> p = params<T, R>(a);
-  if (b.grid)
-    MK_TRY(launch<S>(norm_bwd<T, R, V, ITEMS, S>, b.grid, b.block, Column<T, R, V, ITEMS, true>::kPieces,
-                     3 * a->D * sizeof(float), s,
-                     "mk_block_norm_grad: launch", p));
+  const auto kernel = norm_bwd<T, R, V, ITEMS, THREADS, BLOCKS>;
+  const size_t smem = (size_t)3 * V * ITEMS * sizeof(float) * b.block.x * b.block.y;
+  MK_TRY(mk::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem));
+  if (b.grid) kernel<<<(unsigned)b.grid, b.block, smem, s>>>(p);
   norm_fold<<<(unsigned)mk::cdiv(3 * a->D, 32), dim3(32, 8), 0, s>>>(p.parts, b.parts, a->D, a->dw, a->dhw, a->dscale);
   return mk::check_launch("mk_block_norm_grad: launch");
 }
 
 template <typename T, typename R>
 int run_bwd(const mk_norm_args* a, const BwdPlan& b, cudaStream_t s) {
-  if constexpr (sizeof(T) == 2) {
-    if (b.V == 8) return b.items == 1 ? launch_bwd<T, R, 8, 1, 3>(a, b, s) : launch_bwd<T, R, 8, 2, 1>(a, b, s);
-  } else {
-    if (b.V == 4) return b.items == 2 ? launch_bwd<T, R, 4, 2, 2>(a, b, s) : launch_bwd<T, R, 4, 4, 1>(a, b, s);
-  }
-  return b.items == 4 ? launch_bwd<T, R, 1, 4, 1>(a, b, s) : launch_bwd<T, R, 1, 16, 1>(a, b, s);
+  constexpr int V = sizeof(T) == 2 ? 8 : 4;
+  if (a->D > 4096)
+    return b.V == V ? launch_bwd<T, R, V, 16 / V, 1024, 1>(a, b, s) : launch_bwd<T, R, 1, 16, 1024, 1>(a, b, s);
+  return b.V == V ? launch_bwd<T, R, V, 8 / V, 512, 1>(a, b, s) : launch_bwd<T, R, 1, 8, 512, 1>(a, b, s);
 }
 
 int forward(const mk_norm_args* a, void* stream) {
   MK_TRY(check("mk_block_norm", a, false));
   if (a->T == 0) return MK_OK;
   MK_ENTRY_DEVICE(dev);
+  (void)dev;
   cudaStream_t s = mk::as_stream(stream);
-  if (a->type == MK_T_F32) return run_fwd<float, float>(a, dev, s);
+  if (a->type == MK_T_F32) return run_fwd<float, float>(a, s);
   if (a->type == MK_T_F16)
-    return a->rtype == MK_T_F32 ? run_fwd<__half, float>(a, dev, s) : run_fwd<__half, __half>(a, dev, s);
-  return a->rtype == MK_T_F32 ? run_fwd<__nv_bfloat16, float>(a, dev, s)
-                              : run_fwd<__nv_bfloat16, __nv_bfloat16>(a, dev, s);
+    return a->rtype == MK_T_F32 ? run_fwd<__half, float>(a, s) : run_fwd<__half, __half>(a, s);
+  return a->rtype == MK_T_F32 ? run_fwd<__nv_bfloat16, float>(a, s)
+                              : run_fwd<__nv_bfloat16, __nv_bfloat16>(a, s);
 }
 
 int workspace(const mk_norm_args* a, size_t* bytes) {

@@ -9,6 +9,8 @@
 // their last W - 1 inputs in registers and walks TT tokens, with the next
 // tokens' loads in flight while it computes.  The W - 1 tokens before a tile are
 // read again (they hit L2), which is all that is read twice.
+#include <type_traits>
+
 #include "tokens.cuh"
 
 namespace {
@@ -81,6 +83,55 @@ __device__ __forceinline__ void check_inputs(const Conv<T>& p, int64_t block, in
   }
 }
 
+// A thread's V channels of a value, in pairs (one channel: half a pair).
+template <int V> constexpr int kPairs = (V + 1) / 2;
+
+template <int V, typename T>
+__device__ __forceinline__ void to_pairs(F2 (&f)[kPairs<V>], const T (&v)[V]) {
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) f[i] = pack(to_f(v[2 * i]), V > 1 ? to_f(v[2 * i + (V > 1)]) : 0.0f);
+}
+template <int V, typename T>
+__device__ __forceinline__ void put_pairs(T* p, const F2 (&f)[kPairs<V>]) {
+  Vec<T, V> r;
+  if constexpr (V > 1) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) from_f2(&r.v[2 * i], f[i]);
+  } else {
+    float a, b;
+    unpack(f[0], a, b);
+    r.v[0] = from_f<T>(a);
+  }
+  *reinterpret_cast<Vec<T, V>*>(p) = r;
+}
+template <int V, bool EXACT>
+__device__ __forceinline__ F2 sigmoid_pair(F2 x) {
+  float a, b;
+  unpack(x, a, b);
+  return pack(sigmoid<EXACT>(a), V > 1 ? sigmoid<EXACT>(b) : 0.0f);
+}
+// w and bias of a thread's channels
+template <typename T, int V, int W>
+__device__ __forceinline__ void load_taps(F2 (&w)[W][kPairs<V>], F2 (&bias)[kPairs<V>], const Conv<T>& p, int64_t d) {
+  float r[V];
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = p.w[k * p.D + d + i];
+    to_pairs<V>(w[k], r);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) r[i] = p.bias ? p.bias[d + i] : 0.0f;
+  to_pairs<V>(bias, r);
+}
+template <typename T, int V, int W>
+__device__ __forceinline__ void load_seen_pairs(F2 (&f)[kPairs<V>], const Conv<T>& p, int64_t d, int64_t at, int64_t lo,
+                                                int64_t row) {
+  float r[V];
+  load_seen<T, V, W>(r, p, d, at, lo, row);
+  to_pairs<V>(f, r);
+}
+
 // A thread's tokens of one matrix, kBatch at a time: kBatches - 1 batches are in
 // flight while one is computed.  Vectors go through a ring in shared memory,
 // single elements (which may be too small to copy) through registers.
@@ -129,13 +180,9 @@ __global__ void __launch_bounds__(kLanes* kRows) conv_fwd(Conv<T> p) {
   const int64_t t0 = tile * p.tt, t1 = min(p.q.T, t0 + p.tt);
   const int64_t s0 = seq_at(p.q, t0);
   if (d >= p.D) return;
-  float w[W][V], bias[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int k = 0; k < W; ++k) w[k][i] = p.w[k * p.D + d + i];
-    bias[i] = p.bias ? p.bias[d + i] : 0.0f;
-  }
+  constexpr int Q = kPairs<V>;
+  F2 w[W][Q], bias[Q];
+  load_taps<T, V, W>(w, bias, p, d);
   int64_t t = t0;
   for (int64_t s = s0; s < p.q.nseq && t < t1; ++s) {
     const Span sp = seq_span(p.q, s);
@@ -146,9 +193,9 @@ __global__ void __launch_bounds__(kLanes* kRows) conv_fwd(Conv<T> p) {
 #pragma unroll
     for (int n = 0; n < kFlight; ++n) x.ask(ring, p.x + d, p.ldx, a + n * kBatch, b, n), copy_commit();
     const int64_t row = p.init ? slot_of(p.slots, p.nslots, s, p.err) : -1;
-    float seen[W - 1][V];  // the last W - 1 inputs
+    F2 seen[W - 1 + kBatch][Q];  // the last W - 1 inputs, then a batch
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k) load_seen<T, V, W>(seen[k], p, d, a - (W - 1) + k, sp.lo, row);
+    for (int k = 0; k < W - 1; ++k) load_seen_pairs<T, V, W>(seen[k], p, d, a - (W - 1) + k, sp.lo, row);
     int n = 0;
     for (t = a; t < b; t += kBatch, ++n) {
       if (X::kRing) {
@@ -160,24 +207,25 @@ __global__ void __launch_bounds__(kLanes* kRows) conv_fwd(Conv<T> p) {
         x.take(ring, n);
         x.ask(ring, p.x + d, p.ldx, t + kBatch, b, n + 1);
       }
+      T* y = p.y + t * p.ldy + d;
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        if (t + j >= b) break;
-        float out[V];
+        to_pairs<V>(seen[W - 1 + j], x.now[j].v);
+        F2 out[Q];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float v = to_f(x.now[j].v[i]);
-          float acc = bias[i];
+        for (int i = 0; i < Q; ++i) {
+          F2 acc = bias[i];
 #pragma unroll
-          for (int k = 0; k < W - 1; ++k) acc = fmaf(w[k][i], seen[k][i], acc);
-          acc = fmaf(w[W - 1][i], v, acc);
-          out[i] = p.silu ? acc * sigmoid<kExact>(acc) : acc;
-#pragma unroll
-          for (int k = 0; k < W - 2; ++k) seen[k][i] = seen[k + 1][i];
-          seen[W - 2][i] = v;
+          for (int k = 0; k < W; ++k) acc = fma2(w[k][i], seen[j + k][i], acc);
+          out[i] = p.silu ? mul2(acc, sigmoid_pair<V, kExact>(acc)) : acc;
         }
-        store<T, V>(p.y + (t + j) * p.ldy + d, out);
+        if (t + j < b) put_pairs<V>(y, out);
+        y += p.ldy;
       }
+#pragma unroll
+      for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < Q; ++i) seen[k][i] = seen[kBatch + k][i];
     }
     copy_wait<0>();
     t = b;
@@ -200,7 +248,7 @@ __global__ void __launch_bounds__(kLanes* kRows) conv_fwd(Conv<T> p) {
 // summed over the tile in registers, over the block's tiles in shared memory,
 // and over blocks by a second launch in a fixed order (no atomics).
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(kLanes* kRows, 3) conv_bwd(Conv<T> p) {
+__global__ void __launch_bounds__(kLanes* kRows, 4) conv_bwd(Conv<T> p) {
   using X = Tokens<T, V, sizeof(T) == 4 ? 2 : 4>;  // two rings of Float32: as many as 48 KB hold
   __shared__ Vec<T, V> ring_x[X::kSlots], ring_dy[X::kSlots];
   __shared__ float sm[kRows][(W + 1) * V][kLanes];
@@ -209,17 +257,19 @@ __global__ void __launch_bounds__(kLanes* kRows, 3) conv_bwd(Conv<T> p) {
   const int64_t tile = (int64_t)blockIdx.x * kRows + threadIdx.y;
   if (blockIdx.y == 0) check_inputs(p, blockIdx.x, gridDim.x, threadIdx.y * kLanes + threadIdx.x, kLanes * kRows);
   constexpr bool kExact = sizeof(T) == 4;
-  float dw[W][V] = {}, db[V] = {};
+  constexpr int Q = kPairs<V>;
+  F2 dw[W][Q], db[Q];
+#pragma unroll
+  for (int i = 0; i < Q; ++i) {
+    db[i] = pack(0.0f);
+#pragma unroll
+    for (int k = 0; k < W; ++k) dw[k][i] = pack(0.0f);
+  }
   const int64_t t0 = tile * p.tt, t1 = min(p.q.T, t0 + p.tt);
   const int64_t s0 = tile < p.tiles ? seq_at(p.q, t0) : 0;
   if (d < p.D && tile < p.tiles) {
-    float w[W][V], bias[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-#pragma unroll
-      for (int k = 0; k < W; ++k) w[k][i] = p.w[k * p.D + d + i];
-      bias[i] = p.bias ? p.bias[d + i] : 0.0f;
-    }
+    F2 w[W][Q], bias[Q];
+    load_taps<T, V, W>(w, bias, p, d);
     int64_t t = t0;
     for (int64_t s = s0; s < p.q.nseq && t < t1; ++s) {
       const Span sp = seq_span(p.q, s);
@@ -234,9 +284,14 @@ __global__ void __launch_bounds__(kLanes* kRows, 3) conv_bwd(Conv<T> p) {
         up.ask(ring_dy, p.dy + d, p.lddy, a + n * kBatch, end, n);
         copy_commit();
       }
-      float seen[W][V], win[W][V] = {};
+      // the last W - 1 inputs and the last W - 1 of dp, each with a batch behind them
+      F2 seen[W - 1 + kBatch][Q], win[W - 1 + kBatch][Q];
 #pragma unroll
-      for (int k = 0; k < W - 1; ++k) load_seen<T, V, W>(seen[k], p, d, a - (W - 1) + k, sp.lo, s);
+      for (int k = 0; k < W - 1; ++k) {
+        load_seen_pairs<T, V, W>(seen[k], p, d, a - (W - 1) + k, sp.lo, s);
+#pragma unroll
+        for (int i = 0; i < Q; ++i) win[k][i] = pack(0.0f);
+      }
       int n = 0;
       for (int64_t c = a; c < stop; c += kBatch, ++n) {
         if (X::kRing) {
@@ -250,61 +305,77 @@ __global__ void __launch_bounds__(kLanes* kRows, 3) conv_bwd(Conv<T> p) {
           x.ask(ring_x, p.x + d, p.ldx, c + kBatch, end, n + 1);
           up.ask(ring_dy, p.dy + d, p.lddy, c + kBatch, end, n + 1);
         }
+        // FULL: every token of the batch is the tile's, and so is every output
+        auto batch = [&](auto full) {
+          constexpr bool FULL = decltype(full)::value;
+          T* dx = p.dx + (c - (W - 1)) * p.lddx + d;
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int64_t at = c + j;
-          if (at >= stop) break;
-          const bool inside = at < sp.hi;
-          float out[V];
+          for (int j = 0; j < kBatch; ++j, dx += p.lddx) {
+            const int64_t at = c + j;
+            const bool inside = FULL || at < sp.hi, counts = FULL || at < b;
+            F2 dp[Q], out[Q];
+            to_pairs<V>(seen[W - 1 + j], x.now[j].v);
+            to_pairs<V>(dp, up.now[j].v);
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            float dp = 0.0f;
-            if (inside) {
-              seen[W - 1][i] = to_f(x.now[j].v[i]);
-              dp = to_f(up.now[j].v[i]);
+            for (int i = 0; i < Q; ++i) {
               if (p.silu) {
-                float pre = bias[i];
+                F2 pre = bias[i];
 #pragma unroll
-                for (int k = 0; k < W; ++k) pre = fmaf(w[k][i], seen[k][i], pre);
-                const float sg = sigmoid<kExact>(pre);
-                dp *= sg * fmaf(pre, 1.0f - sg, 1.0f);
+                for (int k = 0; k < W; ++k) pre = fma2(w[k][i], seen[j + k][i], pre);
+                const F2 sg = sigmoid_pair<V, kExact>(pre);
+                // silu' = s + pre s (1 - s)
+                dp[i] = mul2(dp[i], fma2(mul2(pre, sg), fma2(sg, pack(-1.0f), pack(1.0f)), sg));
               }
-              if (at < b) {
+              if (!inside) dp[i] = pack(0.0f);
+              if (counts) {
 #pragma unroll
-                for (int k = 0; k < W; ++k) dw[k][i] = fmaf(dp, seen[k][i], dw[k][i]);
-                db[i] += dp;
+                for (int k = 0; k < W; ++k) dw[k][i] = fma2(dp[i], seen[j + k][i], dw[k][i]);
+                db[i] = add2(db[i], dp[i]);
               }
+              win[W - 1 + j][i] = dp[i];
+              out[i] = mul2(w[0][i], win[W - 1 + j][i]);
 #pragma unroll
-              for (int k = 0; k < W - 1; ++k) seen[k][i] = seen[k + 1][i];
+              for (int k = 0; k < W - 1; ++k) out[i] = fma2(w[W - 1 - k][i], win[j + k][i], out[i]);
             }
+            if constexpr (FULL) {
+              put_pairs<V>(dx, out);
+            } else {
+              const int64_t o = at - (W - 1);
+              if (at < stop && (o >= a || (a == sp.lo && o >= sp.lo - (W - 1)))) {
+                if (p.dlast && o >= sp.hi - (W - 1)) {
+                  float r[V];
+                  F2 more[Q];
+                  load<T, V>(r, p.dlast + (s * (W - 1) + (o - sp.hi + W - 1)) * p.D + d);
+                  to_pairs<V>(more, r);
 #pragma unroll
-            for (int k = 0; k < W - 1; ++k) win[k][i] = win[k + 1][i];
-            win[W - 1][i] = dp;
-            float acc = 0.0f;
-#pragma unroll
-            for (int k = 0; k < W; ++k) acc = fmaf(w[W - 1 - k][i], win[k][i], acc);
-            out[i] = acc;
+                  for (int i = 0; i < Q; ++i) out[i] = add2(out[i], more[i]);
+                }
+                if (o >= a) put_pairs<V>(dx, out);
+                else if (p.dinit) put_pairs<V>(p.dinit + (s * (W - 1) + (o - sp.lo + W - 1)) * p.D + d, out);
+              }
+            }
           }
-          const int64_t o = at - (W - 1);
-          if (p.dlast && o >= sp.hi - (W - 1) && (o >= a || a == sp.lo)) {
-            float dl[V];
-            load<T, V>(dl, p.dlast + (s * (W - 1) + (o - sp.hi + W - 1)) * p.D + d);
+        };
+        if (c > a && c + kBatch <= b) batch(std::true_type{});
+        else batch(std::false_type{});
 #pragma unroll
-            for (int i = 0; i < V; ++i) out[i] += dl[i];
-          }
-          if (o >= a) store<T, V>(p.dx + o * p.lddx + d, out);
-          else if (a == sp.lo && p.dinit) store<T, V>(p.dinit + (s * (W - 1) + (o - sp.lo + W - 1)) * p.D + d, out);
-        }
+        for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+          for (int i = 0; i < Q; ++i) seen[k][i] = seen[kBatch + k][i], win[k][i] = win[kBatch + k][i];
       }
       copy_wait<0>();
       t = b;
     }
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+  for (int i = 0; i < Q; ++i) {
 #pragma unroll
-    for (int k = 0; k < W; ++k) sm[threadIdx.y][k * V + i][threadIdx.x] = dw[k][i];
-    sm[threadIdx.y][W * V + i][threadIdx.x] = db[i];
+    for (int k = 0; k <= W; ++k) {
+      float e, o;
+      unpack(k < W ? dw[k < W ? k : 0][i] : db[i], e, o);
+      sm[threadIdx.y][k * V + 2 * i][threadIdx.x] = e;
+      if (V > 1) sm[threadIdx.y][k * V + 2 * i + (V > 1)][threadIdx.x] = o;
+    }
   }
   __syncthreads();
   if (d >= p.D) return;

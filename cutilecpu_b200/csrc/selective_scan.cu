@@ -10,7 +10,8 @@ using namespace mk::scan;
 // One token per batch entry.  Bound by the state: read and written once, 16
 // bytes per lane and channel, P lanes per channel in memory order.  A thread
 // takes IT channels, so that as many states are in flight and one read of B
-// and C serves them all.
+// and C serves them all; with IT == P each of the P lanes also computes what
+// one of those channels needs once (softplus, gate), and passes it round.
 template <typename T>
 struct Step {
   int64_t D, N, G, Dg, B, nslots, tiles, tpg;  // channel tiles, and of one group
@@ -24,7 +25,7 @@ struct Step {
   unsigned* err;
 };
 
-__device__ __forceinline__ void load4(float (&h)[4], const float* at, int64_t n0, int64_t N) {
+__device__ __forceinline__ void load4(float (&h)[4], const float* at, int n0, int N) {
   if (N % 4 == 0) {
     const float4 v = n0 < N ? *reinterpret_cast<const float4*>(at + n0) : make_float4(0, 0, 0, 0);
     h[0] = v.x, h[1] = v.y, h[2] = v.z, h[3] = v.w;
@@ -34,7 +35,7 @@ __device__ __forceinline__ void load4(float (&h)[4], const float* at, int64_t n0
   }
 }
 
-__device__ __forceinline__ void store4(float* at, const float (&h)[4], int64_t n0, int64_t N) {
+__device__ __forceinline__ void store4(float* at, const float (&h)[4], int n0, int N) {
   if (N % 4 == 0) {
     if (n0 < N) *reinterpret_cast<float4*>(at + n0) = make_float4(h[0], h[1], h[2], h[3]);
   } else {
@@ -46,54 +47,69 @@ __device__ __forceinline__ void store4(float* at, const float (&h)[4], int64_t n
 
 template <typename T, int P, int IT>
 __global__ void __launch_bounds__(128) scan_step(Step<T> p) {
+  static_assert(IT == 1 || IT == P, "a channel per lane, or one for all");
   constexpr bool kExact = sizeof(T) == 4;
   constexpr int kChannels = 128 / P;  // a block's channels at a time
-  const int64_t e = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
-  const int64_t g = tile / p.tpg, first = tile % p.tpg * (kChannels * IT) + threadIdx.x / P;
-  const int64_t n0 = threadIdx.x % P * 4;
+  const int64_t e = blockIdx.x / p.tiles;
+  const int tile = blockIdx.x % p.tiles, g = tile / p.tpg, lane = threadIdx.x % P;
+  const int first = tile % p.tpg * (kChannels * IT) + threadIdx.x / P, base = g * (int)p.Dg;
+  const int N = (int)p.N, n0 = lane * 4;  // D * N stays below 2^26
   if (tile == 0) check_distinct(p.slots, e, threadIdx.x, 128, p.err);
   const int64_t row = slot_of(p.slots, p.nslots, e, p.err);
   if (row < 0) return;
-  float h[IT][4], A[IT][4], b[4], c[4], dt[IT], u[IT], z[IT];
-  int64_t d[IT];
+  const float* state = p.state + row * p.D * N;
+  float* next = p.next + row * p.D * N;
+  float h[IT][4], A[IT][4], b[4], c[4];
+  int d[IT];
   bool live[IT];
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
     live[i] = first + i * kChannels < p.Dg;
-    d[i] = g * p.Dg + (live[i] ? first + i * kChannels : 0);
-    load4(h[i], p.state + (row * p.D + d[i]) * p.N, n0, p.N);
+    d[i] = base + (live[i] ? first + i * kChannels : 0);
+    load4(h[i], state + d[i] * N, n0, N);
   }
+  // this lane's own channel: what it needs once
+  int own = d[0];
+  bool own_live = live[0];
 #pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    load4(A[i], p.A + d[i] * p.N, n0, p.N);
-    u[i] = to_f(p.u[e * p.ldu + d[i]]);
-    dt[i] = to_f(p.delta[e * p.lddelta + d[i]]) + (p.bias ? p.bias[d[i]] : 0.0f);
-    z[i] = p.z ? to_f(p.z[e * p.ldz + d[i]]) : 0.0f;
-  }
+  for (int i = 1; i < IT; ++i) own = lane == i ? d[i] : own, own_live = lane == i ? live[i] : own_live;
+  const float u = to_f(p.u[e * p.ldu + own]);
+  float dt = to_f(p.delta[e * p.lddelta + own]) + (p.bias ? p.bias[own] : 0.0f);
+  const float z = p.z ? to_f(p.z[e * p.ldz + own]) : 0.0f, skip = p.Dskip ? p.Dskip[own] : 0.0f;
+#pragma unroll
+  for (int i = 0; i < IT; ++i) load4(A[i], p.A + d[i] * N, n0, N);
+  const T *Bm = p.Bm + e * p.ldb + g * N, *Cm = p.Cm + e * p.ldc + g * N;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    b[j] = n0 + j < p.N ? to_f(p.Bm[e * p.ldb + g * p.N + n0 + j]) : 0.0f;
-    c[j] = n0 + j < p.N ? to_f(p.Cm[e * p.ldc + g * p.N + n0 + j]) : 0.0f;
+    b[j] = n0 + j < N ? to_f(Bm[n0 + j]) : 0.0f;
+    c[j] = n0 + j < N ? to_f(Cm[n0 + j]) : 0.0f;
   }
+  if (p.softplus) dt = softplus<kExact>(dt);
+  const float dtu = dt * u;
+  float y[IT], sum[1];
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    if (p.softplus) dt[i] = softplus<kExact>(dt[i]);
-    float y = 0.0f;
+    const float dt_i = IT > 1 ? __shfl_sync(0xffffffffu, dt, i, P) : dt;
+    const float dtu_i = IT > 1 ? __shfl_sync(0xffffffffu, dtu, i, P) : dtu;
+    y[i] = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      h[i][j] = fmaf(decay(dt[i], A[i][j] * kLog2e), h[i][j], dt[i] * u[i] * b[j]);
-      y = fmaf(c[j], h[i][j], y);
+      h[i][j] = fmaf(decay(dt_i, A[i][j] * kLog2e), h[i][j], dtu_i * b[j]);
+      y[i] = fmaf(c[j], h[i][j], y[i]);
     }
-#pragma unroll
-    for (int bit = 1; bit < P; bit *= 2) y += __shfl_xor_sync(0xffffffffu, y, bit);
-    if (!live[i]) continue;
-    store4(p.next + (row * p.D + d[i]) * p.N, h[i], n0, p.N);
-    if (n0 == 0) {
-      y = fmaf(p.Dskip ? p.Dskip[d[i]] : 0.0f, u[i], y);
-      if (p.z) y *= z[i] * sigmoid<kExact>(z[i]);
-      p.y[e * p.ldy + d[i]] = from_f<T>(y);
-    }
+    if (live[i]) store4(next + d[i] * N, h[i], n0, N);
   }
+  if constexpr (IT > 1) {
+    reduce_scatter<IT, P, 1>(y, lane, sum);
+  } else {
+    sum[0] = y[0];
+#pragma unroll
+    for (int bit = 1; bit < P; bit *= 2) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], bit);
+  }
+  if (!own_live || (IT == 1 && lane != 0)) return;
+  float out = fmaf(skip, u, sum[0]);
+  if (p.z) out *= z * sigmoid<kExact>(z);
+  p.y[e * p.ldy + own] = from_f<T>(out);
 }
 
 // ---- host side ----------------------------------------------------------------
@@ -210,13 +226,14 @@ int workspace(const char* who, const mk_scan_args* a, bool grad, size_t* bytes) 
 
 template <typename T, int P>
 int launch_step(Step<T> p, const mk::Device* dev, cudaStream_t s) {
-  // four channels per thread, one where that would leave SMs without a block
-  const int64_t four = p.G * mk::cdiv(p.Dg, 4 * (128 / P));
-  const bool wide = four * p.B >= 2 * (int64_t)dev->sms;
-  p.tpg = wide ? four / p.G : mk::cdiv(p.Dg, 128 / P);
+  // P channels per thread (up to 8), one where that would leave SMs without a block
+  constexpr int IT = P <= 8 ? P : 1;
+  const int64_t few = p.G * mk::cdiv(p.Dg, IT * (128 / P));
+  const bool wide = few * p.B >= 2 * (int64_t)dev->sms;
+  p.tpg = wide ? few / p.G : mk::cdiv(p.Dg, 128 / P);
   p.tiles = p.G * p.tpg;
   const unsigned grid = (unsigned)(p.B * p.tiles);
-  if (wide) scan_step<T, P, 4><<<grid, 128, 0, s>>>(p);
+  if (wide) scan_step<T, P, IT><<<grid, 128, 0, s>>>(p);
   else scan_step<T, P, 1><<<grid, 128, 0, s>>>(p);
   return mk::check_launch("mk_selective_scan_step: launch");
 }

@@ -80,11 +80,6 @@ __device__ __forceinline__ void copy_if(void* smem, const void* p, bool on) {
                  : "memory");
   }
 }
-// 16 bytes, or zeros where not `on` (p is an address that may be read all the same).
-__device__ __forceinline__ void copy_or_zero(void* smem, const void* p, bool on) {
-  const unsigned to = (unsigned)__cvta_generic_to_shared(smem), bytes = on ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(p), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
 __device__ __forceinline__ void copy_wait() {

@@ -34,7 +34,7 @@ import math
 import torch
 
 from . import _lib
-from .array import MLIRArray, MLIRCUDABackend, MLIRRows, allocate, current_stream_handle, on_device
+from .array import MLIRArray, MLIRCUDABackend, MLIRRows, allocate, launch, on_device
 
 _FLOATS = ("Float32", "Float16", "BFloat16")
 
@@ -46,43 +46,80 @@ def _fail(what: str, msg: str):
 class _Call:
     """Checks the arrays of one call and collects what the C entry point takes."""
 
+    __slots__ = ("what", "arrays", "eltype", "lead")
+
     def __init__(self, what: str):
-        self.what, self.arrays, self.eltype = what, [], None
+        self.what, self.arrays, self.eltype, self.lead = what, [], None, None
 
     def tokens(self, a, name: str, rows: int | None = None, cols: int | None = None, eltype: str | None = None):
         """A token array as (pointer, ld); its element type is the call's unless given."""
+        if type(a) is MLIRArray and a.dims == self.lead and a.eltype == (eltype or self.eltype):
+            self.arrays.append(a)  # like the call's first array
+            return a.storage.data_ptr(), a.dims[0]
         if not isinstance(a, (MLIRArray, MLIRRows)):
             _fail(self.what, f"`{name}` must be an MLIRArray or rows of one, got {type(a).__name__}")
         if a.eltype not in _FLOATS:
             _fail(self.what, f"`{name}` has element type {a.eltype}, expected {' or '.join(_FLOATS)}")
-        if eltype is None:
-            if self.eltype is None:
-                self.eltype = a.eltype
-            eltype = self.eltype
-        if a.eltype != eltype:
-            _fail(self.what, f"`{name}` has element type {a.eltype}, expected {eltype}")
-        r, n = a.dims[0] if a.dims else 1, math.prod(a.dims[1:])
+        dims = a.dims
+        if self.eltype is None:
+            self.eltype = a.eltype
+        if self.lead is None and len(dims) > 1:
+            self.lead = dims
+        if a.eltype != (eltype or self.eltype):
+            _fail(self.what, f"`{name}` has element type {a.eltype}, expected {eltype or self.eltype}")
+        r = dims[0] if dims else 1
         if rows is not None:
+            n = math.prod(dims[1:])
             # (N, G, T) arrays: the leading dimensions of a token together
-            if r != rows and isinstance(a, MLIRArray) and len(a.dims) > 1 and r * a.dims[1] == rows:
-                r, n = rows, math.prod(a.dims[2:])
+            if r != rows and len(dims) > 1 and r * dims[1] == rows and isinstance(a, MLIRArray):
+                r, n = rows, math.prod(dims[2:])
             if r != rows or n != cols:
-                _fail(self.what, f"`{name}` has dims {a.dims}, expected {rows} x {cols} tokens")
+                _fail(self.what, f"`{name}` has dims {dims}, expected {rows} x {cols} tokens")
         self.arrays.append(a)
-        return a.pointer(), a.ld if isinstance(a, MLIRRows) else r
+        return a.storage.data_ptr(), a.ld if isinstance(a, MLIRRows) else r
 
-    def dense(self, a, name: str, length: int, eltypes=("Float32",)):
+    def like(self, names: str, rows: int, cols: int, *arrays):
+        """The pointers of several token arrays of the call's lead, then their leading dimensions (None, 0: no array)."""
+        lead, eltype, ptrs, lds = self.lead, self.eltype, [], []
+        for i, a in enumerate(arrays):
+            if a is None:
+                ptrs.append(None)
+                lds.append(0)
+            elif type(a) is MLIRArray and a.dims == lead and a.eltype == eltype:
+                self.arrays.append(a)
+                ptrs.append(a.storage.data_ptr())
+                lds.append(rows)
+            else:
+                p, ld = self.tokens(a, names.split()[i], rows, cols)
+                ptrs.append(p)
+                lds.append(ld)
+        return ptrs + lds
+
+    def floats(self, names: str, length: int, *arrays):
+        """The pointers of several Float32 arrays of `length` elements (None: no array)."""
+        out = []
+        for i, a in enumerate(arrays):
+            if a is None:
+                out.append(None)
+            elif type(a) is MLIRArray and a.eltype == "Float32" and a.storage.numel() == length:
+                self.arrays.append(a)
+                out.append(a.storage.data_ptr())
+            else:
+                out.append(self.dense(a, names.split()[i], length))
+        return out
+
+    def dense(self, a, name: str, length: int | None, eltype: str = "Float32"):
         """A dense array of `length` elements (None: any), as a pointer."""
         if a is None:
             return None
-        if not isinstance(a, MLIRArray):
+        if type(a) is not MLIRArray:
             _fail(self.what, f"`{name}` must be an MLIRArray, got {type(a).__name__}")
-        if a.eltype not in eltypes:
-            _fail(self.what, f"`{name}` has element type {a.eltype}, expected {' or '.join(eltypes)}")
-        if length is not None and a.length != length:
+        if a.eltype != eltype:
+            _fail(self.what, f"`{name}` has element type {a.eltype}, expected {eltype}")
+        if length is not None and a.storage.numel() != length:
             _fail(self.what, f"`{name}` has {a.length} elements, expected {length}")
         self.arrays.append(a)
-        return a.pointer()
+        return a.storage.data_ptr()
 
     def sequences(self, x, seqs):
         """(T, nseq, len, pointer of seqs) of the token array x."""
@@ -90,55 +127,61 @@ class _Call:
         T = math.prod(dims[1:])
         if seqs is None:
             return T, math.prod(dims[2:]), dims[1], None
-        p = self.dense(seqs, "seqs", None, ("Int32",))
+        p = self.dense(seqs, "seqs", None, "Int32")
         if seqs.length < 1:
             _fail(self.what, "`seqs` has no entries, expected one more than sequences")
         return T, seqs.length - 1, 0, p
 
-    def pool(self, name: str, a, slots, one: int, count: int, eltypes=("Float32",)):
+    def pool(self, name: str, a, slots, one: int, count: int, eltype: str = "Float32"):
         """A state array of `count` states of `one` elements, or a pool of any number with slots."""
         if a is None:
             return None, 0
         if slots is None:
-            return self.dense(a, name, one * count, eltypes), count
-        p = self.dense(a, name, None, eltypes)
-        if a.length % one:
+            return self.dense(a, name, one * count, eltype), count
+        p = self.dense(a, name, None, eltype)
+        n, rest = divmod(a.storage.numel(), one)
+        if rest:
             _fail(self.what, f"`{name}` has {a.length} elements, not a number of states of {one}")
-        return p, a.length // one
+        return p, n
 
-    def slots(self, slots, count: int, *pools):
-        """(pointer, number of slots) for the pools given as (name, size or None)."""
+    def slots(self, slots, count: int, first: int | None, second: int | None):
+        """(pointer, number of slots) for the sizes of the two pools (None: no such pool)."""
         if slots is None:
             return None, 0
-        p = self.dense(slots, "slots", count, ("Int32",))
-        sizes = {n for n in pools if n is not None}
-        if len(sizes) > 1:
-            _fail(self.what, f"the state pools hold different numbers of states: {sorted(sizes)}")
-        return p, sizes.pop() if sizes else 0
+        if first is not None and second is not None and first != second:
+            _fail(self.what, f"the state pools hold different numbers of states: {sorted((first, second))}")
+        return self.dense(slots, "slots", count, "Int32"), second if first is None else first
 
     def run(self, entry: str, args, workspace: str | None = None):
         L = _lib.lib()
-        with on_device(*self.arrays):
-            if workspace is not None:
-                n = C.c_size_t()
-                _lib.check(getattr(L, workspace)(args, n), self.what)
-                if n.value:
-                    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
-                    args.workspace, args.workspace_bytes = ws.data_ptr(), n.value
-            _lib.check(getattr(L, entry)(args, current_stream_handle()), self.what)
+        if workspace is None:
+            launch(getattr(L, entry), args, self.arrays, self.what)
+            return
+        query, call, n = getattr(L, workspace), getattr(L, entry), C.c_size_t()
+
+        def both(args, stream):
+            rc = query(args, n)
+            if rc or not n.value:
+                return rc or call(args, stream)
+            ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+            args.workspace, args.workspace_bytes = ws.data_ptr(), n.value
+            return call(args, stream)
+
+        launch(both, args, self.arrays, self.what)
 
 
 # ---- causal convolution ----------------------------------------------------------
 
-def _conv(call: _Call, x, w, bias, silu, seqs):
+def _conv(call: _Call, x, w, silu, seqs):
+    """The first fields of ConvArgs up to seqs, and (D, T, nseq, W, x's pointer and ld, w's pointer)."""
     px, ldx = call.tokens(x, "x")
     T, nseq, ln, pseqs = call.sequences(x, seqs)
     D = x.dims[0]
     pw = call.dense(w, "w", None)
     if w is None or len(w.dims) != 2 or w.dims[0] != D:
         _fail(call.what, f"`w` must be ({D}, taps)")
-    return _lib.ConvArgs(type=_lib.MK_T[call.eltype], width=w.dims[1], silu=int(bool(silu)), D=D, T=T, nseq=nseq,
-                         len=ln, seqs=pseqs, x=px, ldx=ldx, w=pw, bias=call.dense(bias, "bias", D))
+    W = w.dims[1]
+    return (_lib.MK_T[call.eltype], W, 1 if silu else 0, D, T, nseq, ln, pseqs), (D, T, nseq, W, px, ldx, pw)
 
 
 def causal_conv(y, x, w, *, bias=None, silu=True, seqs=None, init=None, last=None, slots=None):
@@ -147,13 +190,14 @@ def causal_conv(y, x, w, *, bias=None, silu=True, seqs=None, init=None, last=Non
     are its state in ``init`` (D, W-1, S), the oldest first, or zero; ``last``
     receives the state behind it and may be ``init``.  ``y`` must not be ``x``."""
     c = _Call("causal_conv")
-    a = _conv(c, x, w, bias, silu, seqs)
-    a.y, a.ldy = c.tokens(y, "y", a.D, a.T)
-    one = a.D * (a.width - 1)
-    a.init, ni = c.pool("init", init, slots, one, a.nseq, (c.eltype,))
-    a.last, nl = c.pool("last", last, slots, one, a.nseq, (c.eltype,))
-    a.slots, a.nslots = c.slots(slots, a.nseq, ni if init is not None else None, nl if last is not None else None)
-    c.run("mk_causal_conv", a)
+    head, (D, T, nseq, W, px, ldx, pw) = _conv(c, x, w, silu, seqs)
+    py, ldy = c.like("y", D, T, y)
+    one = D * (W - 1)
+    pi, ni = c.pool("init", init, slots, one, nseq, c.eltype)
+    pl, nl = c.pool("last", last, slots, one, nseq, c.eltype)
+    pslots, nslots = c.slots(slots, nseq, None if init is None else ni, None if last is None else nl)
+    pb, = c.floats("bias", D, bias)
+    c.run("mk_causal_conv", _lib.ConvArgs(*head, pslots, nslots, px, ldx, py, ldy, pw, pb, pi, pl))
     return y
 
 
@@ -163,16 +207,14 @@ def causal_conv_grad(dx, dw, dy, x, w, *, bias=None, dbias=None, silu=True, seqs
     ``dx``, ``dw`` and, where given, ``dbias`` and ``dinit``.  The forward pass's
     intermediate values are computed again; nothing of it has to be kept."""
     c = _Call("causal_conv_grad")
-    a = _conv(c, x, w, bias, silu, seqs)
-    a.dy, a.lddy = c.tokens(dy, "dy", a.D, a.T)
-    a.dx, a.lddx = c.tokens(dx, "dx", a.D, a.T)
-    one = a.D * (a.width - 1)
-    a.init = c.dense(init, "init", one * a.nseq, (c.eltype,))
-    a.dinit = c.dense(dinit, "dinit", one * a.nseq, (c.eltype,))
-    a.dlast = c.dense(dlast, "dlast", one * a.nseq, (c.eltype,))
-    a.dw = c.dense(dw, "dw", a.D * a.width)
-    a.dbias = c.dense(dbias, "dbias", a.D)
-    c.run("mk_causal_conv_grad", a, "mk_causal_conv_grad_workspace")
+    head, (D, T, nseq, W, px, ldx, pw) = _conv(c, x, w, silu, seqs)
+    pdy, pdx, lddy, lddx = c.like("dy dx", D, T, dy, dx)
+    one = D * (W - 1) * nseq
+    pi, pdl, pdi = (c.dense(a, n, one, c.eltype) for n, a in (("init", init), ("dlast", dlast), ("dinit", dinit)))
+    pdw = c.dense(dw, "dw", D * W)
+    pb, pdb = c.floats("bias dbias", D, bias, dbias)
+    c.run("mk_causal_conv_grad", _lib.ConvArgs(*head, None, 0, px, ldx, None, 0, pw, pb, pi, None, pdy, lddy, pdl, pdx,
+                                               lddx, pdw, pdb, pdi), "mk_causal_conv_grad_workspace")
     return dx
 
 
@@ -188,12 +230,13 @@ def causal_conv_step(y, next, state, x, w, *, bias=None, silu=True, slots=None):
         _fail(c.what, f"`w` must be ({D}, taps)")
     W = w.dims[1]
     py, ldy = c.tokens(y, "y", D, B)
-    ps, ns = c.pool("state", state, slots, max(1, D * (W - 1)), B, (c.eltype,))
-    pn, nn = c.pool("next", next, slots, max(1, D * (W - 1)), B, (c.eltype,))
+    ps, ns = c.pool("state", state, slots, max(1, D * (W - 1)), B, c.eltype)
+    pn, nn = c.pool("next", next, slots, max(1, D * (W - 1)), B, c.eltype)
     pslots, nslots = c.slots(slots, B, ns, nn)
+    # fields in the struct's order
     c.run("mk_causal_conv_step", _lib.ConvStepArgs(
-        type=_lib.MK_T[c.eltype], width=W, silu=int(bool(silu)), D=D, B=B, slots=pslots, nslots=nslots, x=px, ldx=ldx,
-        y=py, ldy=ldy, state=ps, next=pn, w=pw, bias=c.dense(bias, "bias", D)))
+        _lib.MK_T[c.eltype], W, 1 if silu else 0, D, B, pslots, nslots, px, ldx, py, ldy, ps, pn, pw,
+        c.dense(bias, "bias", D)))
     return y
 
 
@@ -205,25 +248,24 @@ def _states(call: _Call, A, B, D: int, T: int):
     if A is None or len(A.dims) != 2 or A.dims[1] != D:
         _fail(call.what, f"`A` must be (states, {D})")
     N = A.dims[0]
-    rows = B.length // T if isinstance(B, (MLIRArray, MLIRRows)) and T else N
+    rows = math.prod(B.dims) // T if T and isinstance(B, (MLIRArray, MLIRRows)) else N
     G = rows // N if N else 0
     if G < 1 or D % G:
         _fail(call.what, f"`B` has dims {getattr(B, 'dims', None)}: not (groups of) {N} rows for {T} tokens")
     return p, N, G
 
 
-def _scan(call: _Call, u, delta, A, B, Cm, D, z, bias, softplus, seqs):
+def _scan(call: _Call, u, delta, A, B, Cm, z, softplus, seqs):
+    """(D, T, N, G, nseq) and the fields of ScanArgs: up to seqs, and from u to A."""
     pu, ldu = call.tokens(u, "u")
     T, nseq, ln, pseqs = call.sequences(u, seqs)
     n = u.dims[0]
-    pd, ldd = call.tokens(delta, "delta", n, T)
     pA, N, G = _states(call, A, B, n, T)
+    pd, pz, ldd, ldz = call.like("delta z", n, T, delta, z)
     pB, ldb = call.tokens(B, "B", G * N, T)
     pC, ldc = call.tokens(Cm, "C", G * N, T)
-    pz, ldz = call.tokens(z, "z", n, T) if z is not None else (None, 0)
-    return _lib.ScanArgs(type=_lib.MK_T[call.eltype], softplus=int(bool(softplus)), D=n, N=N, G=G, T=T, nseq=nseq,
-                         len=ln, seqs=pseqs, u=pu, delta=pd, z=pz, B=pB, C=pC, ldu=ldu, lddelta=ldd, ldz=ldz, ldb=ldb,
-                         ldc=ldc, A=pA, Dskip=call.dense(D, "D", n), bias=call.dense(bias, "bias", n))
+    return ((n, T, N, G, nseq), (_lib.MK_T[call.eltype], 1 if softplus else 0, n, N, G, T, nseq, ln, pseqs),
+            (pu, pd, pz, pB, pC, ldu, ldd, ldz, ldb, ldc, pA))
 
 
 def _saved_length(u, A, T: int, nseq: int) -> int:
@@ -254,14 +296,15 @@ def selective_scan(y, u, delta, A, B, C, *, D=None, z=None, bias=None, softplus=
     ``saved`` (``selective_scan_saved``) keeps what the gradient needs.  ``y`` may be
     ``u``, ``delta`` or ``z``."""
     c = _Call("selective_scan")
-    a = _scan(c, u, delta, A, B, C, D, z, bias, softplus, seqs)
-    a.y, a.ldy = c.tokens(y, "y", a.D, a.T)
-    a.init, ni = c.pool("init", init, slots, a.N * a.D, a.nseq)
-    a.last, nl = c.pool("last", last, slots, a.N * a.D, a.nseq)
-    a.slots, a.nslots = c.slots(slots, a.nseq, ni if init is not None else None, nl if last is not None else None)
-    if saved is not None:
-        a.saved = c.dense(saved, "saved", _saved_length(u, A, a.T, a.nseq))
-    c.run("mk_selective_scan", a, "mk_selective_scan_workspace")
+    (n, T, N, _, nseq), head, inputs = _scan(c, u, delta, A, B, C, z, softplus, seqs)
+    py, ldy = c.like("y", n, T, y)
+    pi, ni = c.pool("init", init, slots, N * n, nseq)
+    pl, nl = c.pool("last", last, slots, N * n, nseq)
+    pslots, nslots = c.slots(slots, nseq, None if init is None else ni, None if last is None else nl)
+    pD, pb = c.floats("D bias", n, D, bias)
+    ps = c.dense(saved, "saved", _saved_length(u, A, T, nseq))
+    c.run("mk_selective_scan", _lib.ScanArgs(*head, pslots, nslots, *inputs, pD, pb, pi, py, ldy, pl, ps),
+          "mk_selective_scan_workspace")
     return y
 
 
@@ -272,25 +315,21 @@ def selective_scan_grad(du, ddelta, dA, dB, dC, dy, u, delta, A, B, C, saved, *,
     ``dbias`` over all tokens.  ``saved`` is what the forward pass left, for the same
     inputs (an ``init`` is in it); ``dD``, ``dz``, ``dbias`` go with ``D``, ``z``, ``bias``."""
     c = _Call("selective_scan_grad")
-    a = _scan(c, u, delta, A, B, C, D, z, bias, softplus, seqs)
-    GN = a.G * a.N
-    a.dy, a.lddy = c.tokens(dy, "dy", a.D, a.T)
-    a.du, a.lddu = c.tokens(du, "du", a.D, a.T)
-    a.ddelta, a.ldddelta = c.tokens(ddelta, "ddelta", a.D, a.T)
-    a.dB, a.lddb = c.tokens(dB, "dB", GN, a.T)
-    a.dC, a.lddc = c.tokens(dC, "dC", GN, a.T)
     for name, given, grad in (("D", D, dD), ("z", z, dz), ("bias", bias, dbias)):
         if (given is None) != (grad is None):
             _fail(c.what, f"`d{name}` is needed exactly when `{name}` is given")
-    if z is not None:
-        a.dz, a.lddz = c.tokens(dz, "dz", a.D, a.T)
-    a.dA = c.dense(dA, "dA", a.N * a.D)
-    a.dDskip = c.dense(dD, "dD", a.D)
-    a.dbias = c.dense(dbias, "dbias", a.D)
-    a.saved = c.dense(saved, "saved", _saved_length(u, A, a.T, a.nseq))
-    a.dinit = c.dense(dinit, "dinit", a.N * a.D * a.nseq)
-    a.dlast = c.dense(dlast, "dlast", a.N * a.D * a.nseq)
-    c.run("mk_selective_scan_grad", a, "mk_selective_scan_grad_workspace")
+    (n, T, N, G, nseq), head, inputs = _scan(c, u, delta, A, B, C, z, softplus, seqs)
+    pdy, pdu, pdd, pdz, lddy, lddu, lddd, lddz = c.like("dy du ddelta dz", n, T, dy, du, ddelta, dz)
+    pdB, lddb = c.tokens(dB, "dB", G * N, T)
+    pdC, lddc = c.tokens(dC, "dC", G * N, T)
+    pD, pb, pdD, pdb = c.floats("D bias dD dbias", n, D, bias, dD, dbias)
+    pdA = c.dense(dA, "dA", N * n)
+    ps = c.dense(saved, "saved", _saved_length(u, A, T, nseq))
+    pdl, pdi = c.floats("dlast dinit", N * n * nseq, dlast, dinit)
+    # fields in the struct's order
+    c.run("mk_selective_scan_grad", _lib.ScanArgs(
+        *head, None, 0, *inputs, pD, pb, None, None, 0, None, ps, pdy, lddy, pdl, pdu, pdd, pdz, pdB, pdC, lddu, lddd,
+        lddz, lddb, lddc, pdA, pdD, pdb, pdi), "mk_selective_scan_grad_workspace")
     return du
 
 
@@ -301,26 +340,27 @@ def selective_scan_step(y, next, state, u, delta, A, B, C, *, D=None, z=None, bi
     as they were."""
     c = _Call("selective_scan_step")
     pu, ldu = c.tokens(u, "u")
-    n, batch = u.dims[0], math.prod(u.dims[1:])
-    pd, ldd = c.tokens(delta, "delta", n, batch)
+    dims = u.dims
+    n, batch = dims[0], dims[1] if len(dims) == 2 else math.prod(dims[1:])
     pA, N, G = _states(c, A, B, n, batch)
     pB, ldb = c.tokens(B, "B", G * N, batch)
     pC, ldc = c.tokens(C, "C", G * N, batch)
-    pz, ldz = c.tokens(z, "z", n, batch) if z is not None else (None, 0)
-    py, ldy = c.tokens(y, "y", n, batch)
+    pd, pz, py, ldd, ldz, ldy = c.like("delta z y", n, batch, delta, z, y)
     ps, ns = c.pool("state", state, slots, N * n, batch)
     pn, nn = c.pool("next", next, slots, N * n, batch)
     pslots, nslots = c.slots(slots, batch, ns, nn)
+    pD, pbias = c.floats("D bias", n, D, bias)
+    # fields in the struct's order
     c.run("mk_selective_scan_step", _lib.ScanStepArgs(
-        type=_lib.MK_T[c.eltype], softplus=int(bool(softplus)), D=n, N=N, G=G, B=batch, slots=pslots, nslots=nslots,
-        u=pu, delta=pd, z=pz, Bmat=pB, Cmat=pC, ldu=ldu, lddelta=ldd, ldz=ldz, ldb=ldb, ldc=ldc, A=pA,
-        Dskip=c.dense(D, "D", n), bias=c.dense(bias, "bias", n), state=ps, next=pn, y=py, ldy=ldy))
+        _lib.MK_T[c.eltype], 1 if softplus else 0, n, N, G, batch, pslots, nslots, pu, pd, pz, pB, pC, ldu, ldd, ldz,
+        ldb, ldc, pA, pD, pbias, ps, pn, py, ldy))
     return y
 
 
 # ---- norms around a block ----------------------------------------------------------
 
 def _norm(call: _Call, r, w, h, hw, gate, scale, act, eps, lead):
+    """NormArgs with the inputs filled in."""
     if act not in _lib.MK_ACT:
         _fail(call.what, f"no gate activation {act!r} (supported: silu, sigmoid)")
     call.tokens(lead, "h" if lead is h else "y")  # sets the call's element type
@@ -329,18 +369,16 @@ def _norm(call: _Call, r, w, h, hw, gate, scale, act, eps, lead):
     rt = r.eltype
     if rt not in ("Float32", call.eltype):
         _fail(call.what, f"`r` has element type {rt}, expected Float32 or {call.eltype}")
-    pr, ldr = call.tokens(r, "r", eltype=rt)
-    D, T = r.dims[0], math.prod(r.dims[1:])
     if h is None and not (gate is None and hw is None and scale is None):
         _fail(call.what, "`gate`, `hw` and `scale` belong to `h`")
-    a = _lib.NormArgs(type=_lib.MK_T[call.eltype], rtype=_lib.MK_T[rt], act=_lib.MK_ACT[act], eps=eps, D=D, T=T, r=pr,
-                      ldr=ldr, hw=call.dense(hw, "hw", D), scale=call.dense(scale, "scale", D),
-                      w=call.dense(w, "w", D))
-    if h is not None:
-        a.h, a.ldh = call.tokens(h, "h", D, T)
-    if gate is not None:
-        a.gate, a.ldgate = call.tokens(gate, "gate", D, T)
-    return a
+    pr, ldr = call.tokens(r, "r", eltype=rt)
+    dims = r.dims
+    D, T = dims[0], dims[1] if len(dims) == 2 else math.prod(dims[1:])
+    ph, pg, ldh, ldg = call.like("h gate", D, T, h, gate)
+    phw, psc, pw = call.floats("hw scale w", D, hw, scale, w)
+    # fields in the struct's order, up to ldgate
+    return _lib.NormArgs(_lib.MK_T[call.eltype], _lib.MK_T[rt], _lib.MK_ACT[act], eps, D, T, pr, ph, pg, phw, psc, pw,
+                         None, None, ldr, ldh, ldg)
 
 
 def block_norm(y, rout, r, w, *, h=None, hw=None, gate=None, act="silu", scale=None, eps=1e-5):
@@ -385,15 +423,11 @@ def block_norm_grad(dr, dw, dy, r, w, *, drout=None, h=None, dh=None, hw=None, d
         if (given is None) != (grad is None):
             _fail(c.what, f"`d{name}` is needed exactly when `{name}` is given")
     a = _norm(c, r, w, h, hw, gate, scale, act, eps, h if h is not None else dy if dy is not None else r)
-    a.dr, a.lddr = c.tokens(dr, "dr", a.D, a.T, eltype=r.eltype)
-    if dy is not None:
-        a.dy, a.lddy = c.tokens(dy, "dy", a.D, a.T)
+    D, T = a.D, a.T
+    a.dr, a.lddr = c.tokens(dr, "dr", D, T, eltype=r.eltype)
+    a.dy, a.dh, a.dgate, a.lddy, a.lddh, a.lddgate = c.like("dy dh dgate", D, T, dy, dh, dgate)
     if drout is not None:
-        a.drout, a.lddrout = c.tokens(drout, "drout", a.D, a.T, eltype=r.eltype)
-    if h is not None:
-        a.dh, a.lddh = c.tokens(dh, "dh", a.D, a.T)
-    if gate is not None:
-        a.dgate, a.lddgate = c.tokens(dgate, "dgate", a.D, a.T)
-    a.dw, a.dhw, a.dscale = c.dense(dw, "dw", a.D), c.dense(dhw, "dhw", a.D), c.dense(dscale, "dscale", a.D)
+        a.drout, a.lddrout = c.tokens(drout, "drout", D, T, eltype=r.eltype)
+    a.dw, a.dhw, a.dscale = c.floats("dw dhw dscale", D, dw, dhw, dscale)
     c.run("mk_block_norm_grad", a, "mk_block_norm_grad_workspace")
     return dr

@@ -315,6 +315,179 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_bwd(Norm<T, R> p) {
   }
 }
 
+// The same for 16-bit columns of up to 4096 channels whose rows are 16-byte
+// vectors, one per thread: a block's registers leave one to an SM, so what
+// hides its waits is not another block but the columns ahead.  S - 1 columns
+// are on their way into shared memory while one is computed (every thread
+// copies and reads back its own pieces, no barrier), the parameters lie there
+// in the threads' order, and mean(h^2) of the next column is reduced together
+// with the present one's last sum: two reductions per column instead of three.
+template <typename T, typename R, int S>
+__global__ void __launch_bounds__(512, 1) norm_bwd_ahead(Norm<T, R> p) {
+  constexpr int V = 8, H = V / 2, kR = V * sizeof(R) / 16, kPieces = 2 * kR + 3;  // h, gate, dy, r, drout
+  extern __shared__ uint4 ahead_smem[];  // [S][piece][thread], then [parameter][2][thread]
+  __shared__ Sums<3> sm;
+  int turn = 0;
+  const int nt = blockDim.x * blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
+  const int d = threadIdx.x * V;
+  const bool mine = d < p.D;
+  const int64_t stride = (int64_t)gridDim.x * blockDim.y;
+  const int64_t walker = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  uint4* stages = ahead_smem + tid;
+  uint4* par = ahead_smem + S * kPieces * nt + tid;
+  const float* given[3] = {p.hw, p.scale, p.w};
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    Vec<float, V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = 1.0f;
+    load_vec<float, V>(r, given[i] + d, given[i] && mine);
+    memcpy(par + 2 * i * nt, &r.v[0], 16), memcpy(par + (2 * i + 1) * nt, &r.v[4], 16);
+  }
+  sm.clear();
+  // pairs 2 q and 2 q + 1 of parameter i
+  auto param = [&](F2 (&f)[2], int i, int q) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(par + (2 * i + q) * nt);
+    f[0].v = v.x, f[1].v = v.y;
+  };
+  auto copy = [&](int64_t t, int stage) {
+    uint4* to = stages + stage * kPieces * nt;
+    const bool on = mine && t < p.T_;
+    copy_or_zero(to, on && p.h ? (const void*)(p.h + t * p.ldh + d) : p.r, on && p.h);
+    copy_or_zero(to + nt, on && p.gate ? (const void*)(p.gate + t * p.ldgate + d) : p.r, on && p.gate);
+    copy_or_zero(to + 2 * nt, on && p.dy ? (const void*)(p.dy + t * p.lddy + d) : p.r, on && p.dy);
+#pragma unroll
+    for (int i = 0; i < kR; ++i) {
+      const int at = d + i * (V / kR);
+      copy_or_zero(to + (3 + i) * nt, on ? (const void*)(p.r + t * p.ldr + at) : p.r, on);
+      copy_or_zero(to + (3 + kR + i) * nt, on && p.drout ? (const void*)(p.drout + t * p.lddrout + at) : p.r,
+                   on && p.drout);
+    }
+    copy_commit();
+  };
+  auto take16 = [&](Vec<T, V> (&r)[1], int stage, int piece) {
+    const uint4 v = read_shared(stages + (stage * kPieces + piece) * nt);
+    memcpy(&r[0], &v, 16);
+  };
+  auto take_r = [&](Vec<R, V> (&r)[1], int stage, int piece) {
+#pragma unroll
+    for (int i = 0; i < kR; ++i) {
+      const uint4 v = read_shared(stages + (stage * kPieces + piece + i) * nt);
+      memcpy(reinterpret_cast<char*>(&r[0]) + 16 * i, &v, 16);
+    }
+  };
+  auto sum_hh = [&](int stage) {
+    Vec<T, V> h[1];
+    take16(h, stage, 0);
+    F2 s = pack(0.0f);
+#pragma unroll
+    for (int j = 0; j < H; ++j) s = fma2(pair_at(h, j), pair_at(h, j), s);
+    return sum2(s);
+  };
+  F2 aw[H], ah[H], as[H];
+#pragma unroll
+  for (int j = 0; j < H; ++j) aw[j] = ah[j] = as[j] = pack(0.0f);
+  const bool silu = p.gate && p.act == MK_ACT_SILU, norm_h = p.h && p.hw;
+  int64_t t = walker;
+  if (t < p.T_) {
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) copy(t + i * stride, i);
+    copy_wait<S - 2>();
+    int n = 0;
+    float i1 = 1.0f;
+    if (norm_h) i1 = rsqrtf(fmaf(column_sum(make_float2(sum_hh(0), 0.0f), sm, turn).x, p.inv_d, p.eps));
+    for (;;) {
+      const F2 i1_2 = pack(i1);
+      F2 x[H], sig[H], sxx = pack(0.0f), sdx = pack(0.0f);
+      // what is read is read again in each part: registers are scarcer than shared memory
+      Vec<T, V> h[1], g[1], dy[1];
+      Vec<R, V> r[1];
+      take16(h, n, 0), take16(g, n, 1), take16(dy, n, 2), take_r(r, n, 3);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {  // without h its values are zeros, without dy those
+        F2 hw[2], sc[2], w[2];
+        param(hw, 0, q), param(sc, 1, q), param(w, 2, q);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int j = 2 * q + i;
+          const F2 gj = pair_at(g, j);
+          sig[j] = p.gate ? sigmoid2<false>(gj) : pack(1.0f);
+          F2 m = mul2(mul2(pair_at(h, j), i1_2), mul2(hw[i], sig[j]));
+          if (silu) m = mul2(m, gj);
+          x[j] = fma2(sc[i], m, pair_at(r, j));
+          sxx = fma2(x[j], x[j], sxx);
+          sdx = fma2(mul2(pair_at(dy, j), w[i]), x[j], sdx);
+        }
+      }
+      float i2 = 0.0f, mean = 0.0f;
+      if (p.dy) {
+        const float2 s = column_sum(make_float2(sum2(sxx), sum2(sdx)), sm, turn);
+        i2 = rsqrtf(fmaf(s.x, p.inv_d, p.eps));
+        mean = s.y * i2 * p.inv_d;
+      }
+      const F2 i2_2 = pack(i2), off = pack(-mean * i2);
+      F2 sdv = pack(0.0f);
+      Vec<T, V> dg[1];
+      take16(h, n, 0), take16(g, n, 1), take16(dy, n, 2);
+      take_r(r, n, 3 + kR);  // drout, and from there dr
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        F2 hw[2], sc[2], w[2];
+        param(hw, 0, q), param(sc, 1, q), param(w, 2, q);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int j = 2 * q + i;
+          const F2 xh = mul2(x[j], i2_2), dyj = pair_at(dy, j), v = mul2(pair_at(h, j), i1_2), n_ = mul2(v, hw[i]);
+          aw[j] = fma2(dyj, xh, aw[j]);
+          const F2 dro = fma2(xh, off, fma2(mul2(dyj, w[i]), i2_2, pair_at(r, j))), dm = mul2(dro, sc[i]);
+          put_pair(r, j, dro);
+          const F2 a = silu ? mul2(sig[j], pair_at(g, j)) : sig[j];
+          as[j] = fma2(dro, mul2(n_, a), as[j]);
+          if (p.gate) put_pair(dg, j, mul2(mul2(dm, n_), act_grad(a, sig[j], silu)));
+          const F2 dn = mul2(dm, a);
+          ah[j] = fma2(dn, v, ah[j]);
+          x[j] = mul2(dn, hw[i]);  // from here: the gradient of v
+          sdv = fma2(x[j], v, sdv);
+        }
+      }
+      if (mine) {
+        *reinterpret_cast<Vec<R, V>*>(p.dr + t * p.lddr + d) = r[0];
+        if (p.gate) *reinterpret_cast<Vec<T, V>*>(p.dgate + t * p.lddgate + d) = dg[0];
+      }
+      const int64_t next = t + stride;
+      copy(next + (S - 2) * stride, n == 0 ? S - 1 : n - 1);
+      copy_wait<S - 2>();
+      const int n_next = n + 1 == S ? 0 : n + 1;
+      float back = 0.0f, i1_next = 1.0f;
+      if (norm_h) {
+        const float2 s = column_sum(make_float2(sum2(sdv), sum_hh(n_next)), sm, turn);
+        back = s.x * p.inv_d * i1;
+        i1_next = rsqrtf(fmaf(s.y, p.inv_d, p.eps));
+      }
+      if (p.h) {
+        const F2 minus = pack(-back);
+        take16(h, n, 0);
+#pragma unroll
+        for (int j = 0; j < H; ++j) put_pair(dg, j, mul2(i1_2, fma2(pair_at(h, j), minus, x[j])));
+        if (mine) *reinterpret_cast<Vec<T, V>*>(p.dh + t * p.lddh + d) = dg[0];
+      }
+      t = next;
+      if (t >= p.T_) break;
+      i1 = i1_next, n = n_next;
+    }
+    copy_wait<0>();
+  }
+  float* part = p.parts + walker * 3 * p.D + d;
+  if (!mine) return;
+  Vec<float, V> out[1];
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+#pragma unroll
+    for (int j = 0; j < H; ++j) put_pair(out, j, i == 0 ? aw[j] : i == 1 ? ah[j] : as[j]);
+    *reinterpret_cast<Vec<float, V>*>(part + i * p.D) = out[0];
+  }
+}
+
 // dw, dhw, dscale: the sums over the column walkers, 32 values and 8 ranges of
 // walkers per block.
 __global__ void __launch_bounds__(256) norm_fold(const float* parts, int64_t nparts, int64_t D, float* dw, float* dhw,
@@ -466,11 +639,29 @@ int launch_bwd(const mk_norm_args* a, const BwdPlan& b, cudaStream_t s) {
 }
 
 template <typename T, typename R>
+int launch_bwd_ahead(const mk_norm_args* a, const BwdPlan& b, cudaStream_t s) {
+  constexpr int S = 3;
+  const Norm<T, R> p = params<T, R>(a);
+  const auto kernel = norm_bwd_ahead<T, R, S>;
+  const size_t smem = (size_t)(S * (2 * 8 * sizeof(R) / 16 + 3) + 6) * 16 * b.block.x * b.block.y;
+  MK_TRY(mk::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem));
+  if (b.grid) kernel<<<(unsigned)b.grid, b.block, smem, s>>>(p);
+  norm_fold<<<(unsigned)mk::cdiv(3 * a->D, 32), dim3(32, 8), 0, s>>>(p.parts, b.parts, a->D, a->dw, a->dhw, a->dscale);
+  return mk::check_launch("mk_block_norm_grad: launch");
+}
+
+template <typename T, typename R>
 int run_bwd(const mk_norm_args* a, const BwdPlan& b, cudaStream_t s) {
   constexpr int V = sizeof(T) == 2 ? 8 : 4;
+  if constexpr (V == 8) {
+    if (b.V == 8 && a->D <= 4096) return launch_bwd_ahead<T, R>(a, b, s);
+  }
   if (a->D > 4096)
     return b.V == V ? launch_bwd<T, R, V, 16 / V, 1024, 1>(a, b, s) : launch_bwd<T, R, 1, 16, 1024, 1>(a, b, s);
-  return b.V == V ? launch_bwd<T, R, V, 8 / V, 512, 1>(a, b, s) : launch_bwd<T, R, 1, 8, 512, 1>(a, b, s);
+  if constexpr (V == 4) {
+    if (b.V == 4) return launch_bwd<T, R, 4, 2, 512, 1>(a, b, s);
+  }
+  return launch_bwd<T, R, 1, 8, 512, 1>(a, b, s);
 }
 
 int forward(const mk_norm_args* a, void* stream) {

@@ -80,6 +80,19 @@ __device__ __forceinline__ void copy_if(void* smem, const void* p, bool on) {
                  : "memory");
   }
 }
+// 16 bytes of shared memory, read where it is written (not kept in registers from an earlier read).
+__device__ __forceinline__ uint4 read_shared(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"((unsigned)__cvta_generic_to_shared(p)));
+  return v;
+}
+// 16 bytes, or zeros where not `on` (p is an address that may be read all the same).
+__device__ __forceinline__ void copy_or_zero(void* smem, const void* p, bool on) {
+  const unsigned to = (unsigned)__cvta_generic_to_shared(smem), bytes = on ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(p), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
 __device__ __forceinline__ void copy_wait() {

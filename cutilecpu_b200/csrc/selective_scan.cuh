@@ -661,6 +661,7 @@ struct BwdSmem {
   alignas(16) float B[kTS * Orders<NS, P>::kRow], C[kTS * Orders<NS, P>::kRow];
   unsigned long long sub[kTS / kBwdGroup<P, CH> - 1][CH][NS / 2][kThreads];
   float red[2][kWarps][kBwdGroup<P, CH>][2][NP];
+  float par[2][CB];            // bias and D of the block's channels
   float acc[2][CB][kWarps];    // sums for D and bias, at the end
 };
 
@@ -711,7 +712,7 @@ __device__ __forceinline__ void reduce_channels(F2 (&vB)[NS / 2], F2 (&vC)[NS / 
 }
 
 template <typename T, int NS, int P, int CH, bool VEC>
-__global__ void __launch_bounds__(kThreads, NS * CH <= 4 ? 4 : 2) scan_bwd(Scan<T> p) {
+__global__ void __launch_bounds__(kThreads, CH == 1 && NS <= 4 ? 4 : NS == 2 ? 3 : 2) scan_bwd(Scan<T> p) {
   using W = Place<NS, P, CH>;
   constexpr int NP = W::NP, CB = W::CB, R = W::R, H = NS / 2, K = kBwdGroup<P, CH>;
   constexpr int V = VEC ? 16 / sizeof(T) : 1;
@@ -747,8 +748,25 @@ __global__ void __launch_bounds__(kThreads, NS * CH <= 4 ? 4 : 2) scan_bwd(Scan<
   constexpr int kRow = Orders<NS, P>::kRow;
   const float* lB = sm.B + m * Orders<NS, P>::kStride + n0;
   const float* lC = sm.C + m * Orders<NS, P>::kStride + n0;
+  for (int i = threadIdx.x; i < CB; i += kThreads) {
+    sm.par[0][i] = p.bias && i < w.left ? p.bias[w.base + i] : 0.0f;
+    sm.par[1][i] = p.Dskip && i < w.left ? p.Dskip[w.base + i] : 0.0f;
+  }
+  auto par_pair = [&](int which, int ch) {
+    if constexpr (E == 2) return F2{*reinterpret_cast<const unsigned long long*>(&sm.par[which][ch])};
+    else return pack(sm.par[which][ch], 0.0f);
+  };
+  __syncthreads();
+  // a thread's sums of dB and dC over the warps: which, token of the group and state, and where they go
+  constexpr int kSums = 2 * K * NP / kThreads > 0 ? 2 * K * NP / kThreads : 1;
   int rb = 0;
   const int64_t GN = p.G * p.N;
+  float* part_at[kSums];
+#pragma unroll
+  for (int x = 0; x < kSums; ++x) {
+    const int i = x * kThreads + threadIdx.x, k = i / (2 * NP), which = i / NP % 2, n = i % NP;
+    part_at[x] = p.parts + ((which * p.tpg + w.tg) * p.q.T + k) * GN + w.g * p.N + n;
+  }
   auto load_raw = [&](RawBwd<T, V, S::NV>& r, int64_t tc, int64_t te) {
 #pragma unroll
     for (int i = 0; i < S::NV; ++i) {
@@ -783,23 +801,32 @@ __global__ void __launch_bounds__(kThreads, NS * CH <= 4 ? 4 : 2) scan_bwd(Scan<
       }
     }
     const int64_t piece0 = first_piece(p.q, it.s, kTS);
-    for (int64_t ch = (it.t1 - it.t0 + kTS - 1) / kTS - 1; ch >= 0; --ch) {
+    const int64_t last_tile = (it.t1 - it.t0 + kTS - 1) / kTS - 1;
+    RawBwd<T, V, S::NV> raw, next;
+    Fetched<NP, T> fB, fC;
+    F2 h[CH][H];
+    // what a tile reads: asked for behind the recurrence of the tile before, whose registers are free then (vectors;
+    // single elements take a register each, so they are asked for when they are due)
+    auto ask = [&](int64_t ch) {
       const int64_t tc = it.t0 + ch * kTS, te = min(it.t1, tc + kTS);
-      const int nsub = (int)((te - tc + K - 1) / K);
-      // everything that the tile reads is asked for at once, and the next tile's is called into L2
-      RawBwd<T, V, S::NV> raw;
-      Fetched<NP, T> fB, fC;
-      load_raw(raw, tc, te);
+      load_raw(next, tc, te);
       fB.fetch(p.B, p.ldb, w.g * p.N, p.N, tc, te, p.vec_bc);
       fC.fetch(p.C, p.ldc, w.g * p.N, p.N, tc, te, p.vec_bc);
-      F2 h[CH][H], dAc[CH][H];  // dAc: the tile's sum, so that long sums stay exact
       const float* sv = p.saved + (piece0 + (tc - it.lo) / kTS) * p.D * p.N;
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        load_states<NS>(h[i], sv + w.d[i] * p.N, n0, p.N, m);
+      for (int i = 0; i < CH; ++i) load_states<NS>(h[i], sv + w.d[i] * p.N, n0, p.N, m);
+    };
+    if (VEC && last_tile >= 0) ask(last_tile);
+    for (int64_t ch = last_tile; ch >= 0; --ch) {
+      const int64_t tc = it.t0 + ch * kTS, te = min(it.t1, tc + kTS);
+      const int nsub = (int)((te - tc + K - 1) / K);
+      F2 dAc[CH][H];  // the tile's sum, so that long sums stay exact
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
 #pragma unroll
         for (int j = 0; j < H; ++j) dAc[i][j] = pack(0.0f, 0.0f);
-      }
+      if (!VEC) ask(ch);
+      raw = next;
       if (ch > 0) {
 #pragma unroll
         for (int i = 0; i < S::NV; ++i) {
@@ -811,7 +838,8 @@ __global__ void __launch_bounds__(kThreads, NS * CH <= 4 ? 4 : 2) scan_bwd(Scan<
           if (p.z) prefetch_l2(p.z + t * p.ldz + d);
         }
 #pragma unroll
-        for (int i = 0; i < CH; ++i) prefetch_l2(sv - p.D * p.N + w.d[i] * p.N + (n0 < p.N ? n0 : 0));
+        for (int i = 0; i < CH; ++i)
+          prefetch_l2(p.saved + ((piece0 + (tc - it.lo) / kTS - 1) * p.D + w.d[i]) * p.N + (n0 < p.N ? n0 : 0));
       }
 #pragma unroll
       for (int i = 0; i < S::NV; ++i) {
@@ -822,7 +850,7 @@ __global__ void __launch_bounds__(kThreads, NS * CH <= 4 ? 4 : 2) scan_bwd(Scan<
           float2 x[2], y[2];
           x[0] = x[1] = y[0] = y[1] = make_float2(0.0f, 0.0f);
           if (in) {
-            F2 dt = add2(pair_of<E>(raw.delta[i].v + e), channel_pair<E>(p.bias, w.base, S::col() + e, w.left));
+            F2 dt = add2(pair_of<E>(raw.delta[i].v + e), par_pair(0, S::col() + e));
             F2 dyp = pair_of<E>(raw.dy[i].v + e);
             if (p.softplus) dt = softplus2<kExact>(dt);
             if (p.z) {
@@ -935,13 +963,15 @@ __global__ void __launch_bounds__(kThreads, NS * CH <= 4 ? 4 : 2) scan_bwd(Scan<
         }
         if (q == 0) load_raw(raw, tc, te);  // again, for what is left to do
         __syncthreads();
-        for (int i = threadIdx.x; i < 2 * K * NP; i += kThreads) {
-          const int k = i / (2 * NP), which = i / NP % 2, n = i % NP;
+#pragma unroll
+        for (int x = 0; x < kSums; ++x) {
+          const int i = x * kThreads + threadIdx.x, k = i / (2 * NP), which = i / NP % 2, n = i % NP;
+          if (i >= 2 * K * NP) continue;
           float v = 0.0f;
 #pragma unroll
-          for (int x = 0; x < kWarps; ++x) v += sm.red[rb][x][k][which][n];
-          const int64_t t = tc + q * K + k;
-          if (t < te && n < p.N) p.parts[((which * p.tpg + w.tg) * p.q.T + t) * GN + w.g * p.N + n] = v;
+          for (int y = 0; y < kWarps; ++y) v += sm.red[rb][y][k][which][n];
+          const int64_t t = tc + q * K;
+          if (t + k < te && n < p.N) part_at[x][t * GN] = v;
         }
         rb ^= 1;
       }
@@ -949,6 +979,7 @@ __global__ void __launch_bounds__(kThreads, NS * CH <= 4 ? 4 : 2) scan_bwd(Scan<
       for (int i = 0; i < CH; ++i)
 #pragma unroll
         for (int j = 0; j < H; ++j) dA[i][j] = add2(dA[i][j], dAc[i][j]);
+      if (VEC && ch > 0) ask(ch - 1);
       float add[2 * V] = {};
 #pragma unroll
       for (int i = 0; i < S::NV; ++i) {
@@ -961,7 +992,7 @@ __global__ void __launch_bounds__(kThreads, NS * CH <= 4 ? 4 : 2) scan_bwd(Scan<
           const float2 x0 = sm.X[c], y0 = sm.Y[c], x1 = sm.X[c + E - 1], y1 = sm.Y[c + E - 1];
           const F2 dt = pack(x0.x, x1.x), G = pack(x0.y, x1.y), Tq = pack(y0.x, y1.x);
           const F2 u = pair_of<E>(raw.u[i].v + e), dy = pair_of<E>(raw.dy[i].v + e);
-          const F2 skip = channel_pair<E>(p.Dskip, w.base, S::col() + e, w.left);
+          const F2 skip = par_pair(1, S::col() + e);
           F2 dyp = dy;
           if (p.z) {
             const F2 z = pair_of<E>(raw.z[i].v + e), one = pack(1.0f);
@@ -978,8 +1009,7 @@ __global__ void __launch_bounds__(kThreads, NS * CH <= 4 ? 4 : 2) scan_bwd(Scan<
           F2 dd2 = fma2(u, G, mul2(Tq, pack(kLn2)));
           if (p.softplus) {
             F2 g;
-            softplus2<kExact, true>(
-                add2(pair_of<E>(raw.delta[i].v + e), channel_pair<E>(p.bias, w.base, S::col() + e, w.left)), &g);
+            softplus2<kExact, true>(add2(pair_of<E>(raw.delta[i].v + e), par_pair(0, S::col() + e)), &g);
             dd2 = mul2(dd2, g);
           }
           out_pair<E>(dd.v + e, dd2);

@@ -692,8 +692,8 @@ int gradient(const mk_norm_args* a, void* stream) {
   MK_ENTRY_DEVICE(dev);
   const BwdPlan b = plan_bwd(a, dev);
   const size_t need = (size_t)b.parts * 3 * a->D * sizeof(float);
-  if (need && (!a->workspace || a->workspace_bytes < need || !elem_aligned(a->workspace, 4)))
-    return bad(who, "a workspace of " + std::to_string(need) + " bytes is needed");
+  if (need && (!a->workspace || a->workspace_bytes < need || !elem_aligned(a->workspace, 16)))
+    return bad(who, "a 16-byte aligned workspace of " + std::to_string(need) + " bytes is needed");
   cudaStream_t s = mk::as_stream(stream);
   if (a->type == MK_T_F32) return run_bwd<float, float>(a, b, s);
   if (a->type == MK_T_F16)

@@ -188,7 +188,8 @@ __global__ void __launch_bounds__(kLanes* kRows) conv_fwd(Conv<T> p) {
     const Span sp = seq_span(p.q, s);
     if (sp.hi <= t) continue;
     const int64_t a = max(t, sp.lo), b = min(t1, sp.hi);
-    if (a >= b) break;
+    if (sp.lo >= t1) break;
+    if (a >= b) continue;  // an empty one behind columns of none
     X x;
 #pragma unroll
     for (int n = 0; n < kFlight; ++n) x.ask(ring, p.x + d, p.ldx, a + n * kBatch, b, n), copy_commit();
@@ -275,7 +276,8 @@ __global__ void __launch_bounds__(kLanes* kRows, 4) conv_bwd(Conv<T> p) {
       const Span sp = seq_span(p.q, s);
       if (sp.hi <= t) continue;
       const int64_t a = max(t, sp.lo), b = min(t1, sp.hi);
-      if (a >= b) break;
+      if (sp.lo >= t1) break;
+      if (a >= b) continue;  // an empty one behind columns of none
       const int64_t stop = b + W - 1, end = min(stop, sp.hi);
       X x, up;
 #pragma unroll
@@ -654,8 +656,8 @@ int gradient(const mk_conv_args* a, void* stream) {
   BwdPlan b = plan_bwd(a, dev);
   if (a->nseq == 0) b.parts = b.tiles = 0;
   const size_t need = (size_t)b.parts * (a->width + 1) * a->D * sizeof(float);
-  if (need && (!a->workspace || a->workspace_bytes < need || !elem_aligned(a->workspace, 4)))
-    return bad(who, "a workspace of " + std::to_string(need) + " bytes is needed");
+  if (need && (!a->workspace || a->workspace_bytes < need || !elem_aligned(a->workspace, 16)))
+    return bad(who, "a 16-byte aligned workspace of " + std::to_string(need) + " bytes is needed");
   return dispatch(a->type, a->width, b.V > 1, BwdOp{a, dev, mk::as_stream(stream), b});
 }
 

@@ -276,6 +276,42 @@ __device__ __forceinline__ void out_pair(T* p, F2 x) {
   }
 }
 
+// Two values of a channel and of its neighbour (E == 2) in their cells; zeros where not `in`.
+struct Cell {
+  F2 a, b;
+};
+template <int E>
+__device__ __forceinline__ void put_cell(float2* cell, F2 a, F2 b, bool in, bool there) {
+  float a0, a1, b0, b1;
+  unpack(a, a0, a1), unpack(b, b0, b1);
+  if (!in) a0 = a1 = b0 = b1 = 0.0f;
+  if (!there) return;
+  if constexpr (E == 2) *reinterpret_cast<float4*>(cell) = make_float4(a0, b0, a1, b1);
+  else *cell = make_float2(a0, b0);
+}
+template <int E>
+__device__ __forceinline__ Cell get_cell(const float2* cell) {
+  if constexpr (E == 2) {
+    const float4 v = *reinterpret_cast<const float4*>(cell);
+    return {pack(v.x, v.z), pack(v.y, v.w)};
+  } else {
+    return {pack(cell->x, 0.0f), pack(cell->y, 0.0f)};
+  }
+}
+template <bool EXACT, int E>
+__device__ __forceinline__ F2 softplus_pair(F2 x) {
+  if constexpr (E == 2) return softplus2<EXACT>(x);
+  float a, b;
+  unpack(x, a, b);
+  return pack(softplus<EXACT>(a), 0.0f);
+}
+template <bool EXACT, int E>
+__device__ __forceinline__ F2 sigmoid_pair(F2 x) {
+  float a, b;
+  unpack(x, a, b);
+  return pack(sigmoid<EXACT>(a), E == 2 ? sigmoid<EXACT>(b) : 0.0f);
+}
+
 // The parameters of channel ch of a block (and of the next, E == 2); zero without any.
 template <int E>
 __device__ __forceinline__ F2 channel_pair(const float* p, int64_t base, int ch, int left) {
@@ -364,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
   }
   if (!FULL && it.t1 >= it.hi) return;
   constexpr bool kExact = sizeof(T) == 4;
-  constexpr int E = V > 1 ? 2 : 1;  // values taken at once
+  constexpr int E = V > 1 ? 2 : 1, Q = V / E;  // values taken at once, and how often
   F2 bias[(V + 1) / 2], skip[(V + 1) / 2];
 #pragma unroll
   for (int i = 0; i < V; i += E) {
@@ -381,29 +417,26 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
   float sum_dt[CH] = {};
 
   for (int64_t tt = it.t0; tt < it.t1; tt += kTS) {
+    {
+      // one step for all values at a time: a branch per value would keep them from overlapping
+      F2 dt[S::NV][Q];
 #pragma unroll
-    for (int i = 0; i < S::NV; ++i) {
-      if (!S::has(i)) continue;
-      const bool in = tt + S::row(i) < it.t1 && S::col() < w.left;  // no token: the state stays
+      for (int i = 0; i < S::NV; ++i)
 #pragma unroll
-      for (int e = 0; e < V; e += E) {
-        float2* at_e = cells + cell2<CB>(S::row(i), S::col() + e);
-        if constexpr (E == 2) {
-          F2 dt = add2(to_f2(cur.delta[i].v + e), bias[e / 2]);
-          if (p.softplus) dt = softplus2<kExact>(dt);
-          const F2 dtu = mul2(dt, to_f2(cur.u[i].v + e));
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (in) unpack(dt, v.x, v.z), unpack(dtu, v.y, v.w);
-          *reinterpret_cast<float4*>(at_e) = v;
-        } else {
-          float2 v = make_float2(0.0f, 0.0f);
-          if (in) {
-            v.x = to_f(cur.delta[i].v[0]) + sum2(bias[0]);
-            if (p.softplus) v.x = softplus<kExact>(v.x);
-            v.y = v.x * to_f(cur.u[i].v[0]);
-          }
-          *at_e = v;
-        }
+        for (int e = 0; e < Q; ++e) dt[i][e] = add2(pair_of<E>(cur.delta[i].v + e * E), bias[e]);
+      if (p.softplus) {
+#pragma unroll
+        for (int i = 0; i < S::NV; ++i)
+#pragma unroll
+          for (int e = 0; e < Q; ++e) dt[i][e] = softplus_pair<kExact, E>(dt[i][e]);
+      }
+#pragma unroll
+      for (int i = 0; i < S::NV; ++i) {
+        const bool in = tt + S::row(i) < it.t1 && S::col() < w.left;  // no token: the state stays
+#pragma unroll
+        for (int e = 0; e < Q; ++e)
+          put_cell<E>(cells + cell2<CB>(S::row(i), S::col() + e * E), dt[i][e],
+                      mul2(dt[i][e], pair_of<E>(cur.u[i].v + e * E)), in, S::has(i));
       }
     }
     fB.put(&sB[0][0]);
@@ -479,29 +512,21 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
       for (int i = 0; i < S::NV; ++i) {
         const int64_t t = tt + S::row(i);
         if (!S::has(i) || t >= it.t1 || S::col() >= w.left) continue;
-        Vec<T, V> out;
+        F2 y[Q];
 #pragma unroll
-        for (int e = 0; e < V; e += E) {
-          const float2* at_e = cells + cell2<CB>(S::row(i), S::col() + e);
-          if constexpr (E == 2) {
-            const float4 v = *reinterpret_cast<const float4*>(at_e);
-            F2 y = fma2(skip[e / 2], to_f2(cur.u[i].v + e), pack(v.x, v.z));
-            if (p.z) {
-              float za, zb;
-              const F2 z = to_f2(cur.z[i].v + e);
-              unpack(z, za, zb);
-              y = mul2(mul2(y, z), pack(sigmoid<kExact>(za), sigmoid<kExact>(zb)));
-            }
-            from_f2(out.v + e, y);
-          } else {
-            float y = fmaf(sum2(skip[0]), to_f(cur.u[i].v[0]), at_e->x);
-            if (p.z) {
-              const float z = to_f(cur.z[i].v[0]);
-              y *= z * sigmoid<kExact>(z);
-            }
-            out.v[0] = from_f<T>(y);
+        for (int e = 0; e < Q; ++e)
+          y[e] = fma2(skip[e], pair_of<E>(cur.u[i].v + e * E),
+                      get_cell<E>(cells + cell2<CB>(S::row(i), S::col() + e * E)).a);
+        if (p.z) {
+#pragma unroll
+          for (int e = 0; e < Q; ++e) {
+            const F2 z = pair_of<E>(cur.z[i].v + e * E);
+            y[e] = mul2(mul2(y[e], z), sigmoid_pair<kExact, E>(z));
           }
         }
+        Vec<T, V> out;
+#pragma unroll
+        for (int e = 0; e < Q; ++e) out_pair<E>(out.v + e * E, y[e]);
         *reinterpret_cast<Vec<T, V>*>(p.y + t * p.ldy + w.base + S::col()) = out;
       }
     }
@@ -560,7 +585,7 @@ __global__ void __launch_bounds__(kThreads) scan_rev(Scan<T> p) {
     for (int j = 0; j < H; ++j) A2[i][j] = mul2(A2[i][j], pack(kLog2e, kLog2e)), e_[i][j] = pack(0.0f, 0.0f);
   }
   constexpr bool kExact = sizeof(T) == 4;
-  constexpr int E = V > 1 ? 2 : 1;
+  constexpr int E = V > 1 ? 2 : 1, Q = V / E;
   F2 bias[(V + 1) / 2];
 #pragma unroll
   for (int i = 0; i < V; i += E) bias[i / 2] = channel_pair<E>(p.bias, w.base, S::col() + i, w.left);
@@ -572,38 +597,36 @@ __global__ void __launch_bounds__(kThreads) scan_rev(Scan<T> p) {
     for (int k = 0; k < KV; ++k) at[i][k] = cell2<CB>(k, w.ch[i]) - k * CB;
   float sum_dt[CH] = {};
   for (; tt >= it.t0; tt -= kTS) {
+    {
+      F2 dt[S::NV][Q], dyp[S::NV][Q];
 #pragma unroll
-    for (int i = 0; i < S::NV; ++i) {
-      if (!S::has(i)) continue;
-      const bool in = tt + S::row(i) < it.t1 && S::col() < w.left;
+      for (int i = 0; i < S::NV; ++i)
 #pragma unroll
-      for (int e = 0; e < V; e += E) {
-        float2* at_e = cells + cell2<CB>(S::row(i), S::col() + e);
-        if constexpr (E == 2) {
-          F2 dt = add2(to_f2(cur.delta[i].v + e), bias[e / 2]), dyp = to_f2(cur.u[i].v + e);
-          if (p.softplus) dt = softplus2<kExact>(dt);
-          if (p.z) {
-            float za, zb;
-            const F2 z = to_f2(cur.z[i].v + e);
-            unpack(z, za, zb);
-            dyp = mul2(mul2(dyp, z), pack(sigmoid<kExact>(za), sigmoid<kExact>(zb)));
-          }
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (in) unpack(dt, v.x, v.z), unpack(dyp, v.y, v.w);
-          *reinterpret_cast<float4*>(at_e) = v;
-        } else {
-          float2 v = make_float2(0.0f, 0.0f);
-          if (in) {
-            v.x = to_f(cur.delta[i].v[0]) + sum2(bias[0]);
-            if (p.softplus) v.x = softplus<kExact>(v.x);
-            v.y = to_f(cur.u[i].v[0]);
-            if (p.z) {
-              const float z = to_f(cur.z[i].v[0]);
-              v.y *= z * sigmoid<kExact>(z);
-            }
-          }
-          *at_e = v;
+        for (int e = 0; e < Q; ++e) {
+          dt[i][e] = add2(pair_of<E>(cur.delta[i].v + e * E), bias[e]);
+          dyp[i][e] = pair_of<E>(cur.u[i].v + e * E);
         }
+      if (p.softplus) {
+#pragma unroll
+        for (int i = 0; i < S::NV; ++i)
+#pragma unroll
+          for (int e = 0; e < Q; ++e) dt[i][e] = softplus_pair<kExact, E>(dt[i][e]);
+      }
+      if (p.z) {
+#pragma unroll
+        for (int i = 0; i < S::NV; ++i)
+#pragma unroll
+          for (int e = 0; e < Q; ++e) {
+            const F2 z = pair_of<E>(cur.z[i].v + e * E);
+            dyp[i][e] = mul2(mul2(dyp[i][e], z), sigmoid_pair<kExact, E>(z));
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < S::NV; ++i) {
+        const bool in = tt + S::row(i) < it.t1 && S::col() < w.left;
+#pragma unroll
+        for (int e = 0; e < Q; ++e)
+          put_cell<E>(cells + cell2<CB>(S::row(i), S::col() + e * E), dt[i][e], dyp[i][e], in, S::has(i));
       }
     }
     fC.put(&sC[0][0]);
@@ -719,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, CH == 1 && NS <= 4 ? 4 : NS == 2 ? 3
   using S = Spread<CB, V>;
   constexpr int M = NS < 4 ? NS : 4;
   constexpr bool kExact = sizeof(T) == 4;
-  constexpr int E = V > 1 ? 2 : 1;
+  constexpr int E = V > 1 ? 2 : 1, Q = V / E;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   BwdSmem<NS, P, CH, V>& sm = *reinterpret_cast<BwdSmem<NS, P, CH, V>*>(smem_raw);
   const int64_t tile = blockIdx.x % p.tiles, item0 = blockIdx.x / p.tiles;
@@ -841,35 +864,39 @@ __global__ void __launch_bounds__(kThreads, CH == 1 && NS <= 4 ? 4 : NS == 2 ? 3
         for (int i = 0; i < CH; ++i)
           prefetch_l2(p.saved + ((piece0 + (tc - it.lo) / kTS - 1) * p.D + w.d[i]) * p.N + (n0 < p.N ? n0 : 0));
       }
+      {
+        // one step for all values at a time: a branch per value would keep them from overlapping
+        F2 dt[S::NV][Q], dyp[S::NV][Q];
 #pragma unroll
-      for (int i = 0; i < S::NV; ++i) {
-        if (!S::has(i)) continue;
-        const bool in = tc + S::row(i) < te && S::col() < w.left;
+        for (int i = 0; i < S::NV; ++i)
 #pragma unroll
-        for (int e = 0; e < V; e += E) {
-          float2 x[2], y[2];
-          x[0] = x[1] = y[0] = y[1] = make_float2(0.0f, 0.0f);
-          if (in) {
-            F2 dt = add2(pair_of<E>(raw.delta[i].v + e), par_pair(0, S::col() + e));
-            F2 dyp = pair_of<E>(raw.dy[i].v + e);
-            if (p.softplus) dt = softplus2<kExact>(dt);
-            if (p.z) {
-              const F2 z = pair_of<E>(raw.z[i].v + e);
-              float za, zb;
-              unpack(z, za, zb);
-              dyp = mul2(mul2(dyp, z), pack(sigmoid<kExact>(za), sigmoid<kExact>(zb)));
-            }
-            unpack(dt, x[0].x, x[1].x);
-            unpack(mul2(dt, pair_of<E>(raw.u[i].v + e)), x[0].y, x[1].y);
-            unpack(dyp, y[0].x, y[1].x);
+          for (int e = 0; e < Q; ++e) {
+            dt[i][e] = add2(pair_of<E>(raw.delta[i].v + e * E), par_pair(0, S::col() + e * E));
+            dyp[i][e] = pair_of<E>(raw.dy[i].v + e * E);
           }
-          const int c = cell2<CB>(S::row(i), S::col() + e);
-          if constexpr (E == 2) {
-            *reinterpret_cast<float4*>(sm.X + c) = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
-            *reinterpret_cast<float4*>(sm.Y + c) = make_float4(y[0].x, 0.0f, y[1].x, 0.0f);
-          } else {
-            sm.X[c] = x[0];
-            sm.Y[c] = y[0];
+        if (p.softplus) {
+#pragma unroll
+          for (int i = 0; i < S::NV; ++i)
+#pragma unroll
+            for (int e = 0; e < Q; ++e) dt[i][e] = softplus_pair<kExact, E>(dt[i][e]);
+        }
+        if (p.z) {
+#pragma unroll
+          for (int i = 0; i < S::NV; ++i)
+#pragma unroll
+            for (int e = 0; e < Q; ++e) {
+              const F2 z = pair_of<E>(raw.z[i].v + e * E);
+              dyp[i][e] = mul2(mul2(dyp[i][e], z), sigmoid_pair<kExact, E>(z));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < S::NV; ++i) {
+          const bool in = tc + S::row(i) < te && S::col() < w.left;
+#pragma unroll
+          for (int e = 0; e < Q; ++e) {
+            const int c = cell2<CB>(S::row(i), S::col() + e * E);
+            put_cell<E>(sm.X + c, dt[i][e], mul2(dt[i][e], pair_of<E>(raw.u[i].v + e * E)), in, S::has(i));
+            put_cell<E>(sm.Y + c, dyp[i][e], pack(0.0f), in, S::has(i));
           }
         }
       }
@@ -986,38 +1013,46 @@ __global__ void __launch_bounds__(kThreads, CH == 1 && NS <= 4 ? 4 : NS == 2 ? 3
         const int64_t t = tc + S::row(i), d = w.base + S::col();
         if (!S::has(i) || t >= te || S::col() >= w.left) continue;
         Vec<T, V> du, dd, dz;
+        F2 dyp[Q];
+        Cell x[Q], y[Q];
 #pragma unroll
-        for (int e = 0; e < V; e += E) {
-          const int c = cell2<CB>(S::row(i), S::col() + e);
-          const float2 x0 = sm.X[c], y0 = sm.Y[c], x1 = sm.X[c + E - 1], y1 = sm.Y[c + E - 1];
-          const F2 dt = pack(x0.x, x1.x), G = pack(x0.y, x1.y), Tq = pack(y0.x, y1.x);
-          const F2 u = pair_of<E>(raw.u[i].v + e), dy = pair_of<E>(raw.dy[i].v + e);
-          const F2 skip = par_pair(1, S::col() + e);
-          F2 dyp = dy;
-          if (p.z) {
-            const F2 z = pair_of<E>(raw.z[i].v + e), one = pack(1.0f);
-            float za, zb;
-            unpack(z, za, zb);
-            const F2 sz = pack(sigmoid<kExact>(za), sigmoid<kExact>(zb));
-            const F2 gz = mul2(z, sz);
-            dyp = mul2(dy, gz);
+        for (int e = 0; e < Q; ++e) {
+          const int c = cell2<CB>(S::row(i), S::col() + e * E);
+          x[e] = get_cell<E>(sm.X + c), y[e] = get_cell<E>(sm.Y + c);  // dt, sum g B; sum g q A2, y
+          dyp[e] = pair_of<E>(raw.dy[i].v + e * E);
+        }
+        if (p.z) {
+#pragma unroll
+          for (int e = 0; e < Q; ++e) {
+            const F2 z = pair_of<E>(raw.z[i].v + e * E), sz = sigmoid_pair<kExact, E>(z), gz = mul2(z, sz);
+            const F2 all = fma2(par_pair(1, S::col() + e * E), pair_of<E>(raw.u[i].v + e * E), y[e].b);
             // silu' = s + z s (1 - s)
-            const F2 grad = fma2(gz, fma2(sz, pack(-1.0f), one), sz);
-            out_pair<E>(dz.v + e, mul2(mul2(dy, fma2(skip, u, pack(y0.y, y1.y))), grad));
+            out_pair<E>(dz.v + e * E, mul2(mul2(dyp[e], all), fma2(gz, fma2(sz, pack(-1.0f), pack(1.0f)), sz)));
+            dyp[e] = mul2(dyp[e], gz);
           }
-          out_pair<E>(du.v + e, fma2(dt, G, mul2(skip, dyp)));
-          F2 dd2 = fma2(u, G, mul2(Tq, pack(kLn2)));
-          if (p.softplus) {
+        }
+        F2 dd2[Q];
+#pragma unroll
+        for (int e = 0; e < Q; ++e) {
+          out_pair<E>(du.v + e * E, fma2(x[e].a, x[e].b, mul2(par_pair(1, S::col() + e * E), dyp[e])));
+          dd2[e] = fma2(pair_of<E>(raw.u[i].v + e * E), x[e].b, mul2(y[e].a, pack(kLn2)));
+        }
+        if (p.softplus) {
+#pragma unroll
+          for (int e = 0; e < Q; ++e) {
             F2 g;
-            softplus2<kExact, true>(add2(pair_of<E>(raw.delta[i].v + e), par_pair(0, S::col() + e)), &g);
-            dd2 = mul2(dd2, g);
+            softplus2<kExact, true>(add2(pair_of<E>(raw.delta[i].v + e * E), par_pair(0, S::col() + e * E)), &g);
+            dd2[e] = mul2(dd2[e], g);
           }
-          out_pair<E>(dd.v + e, dd2);
+        }
+#pragma unroll
+        for (int e = 0; e < Q; ++e) {
+          out_pair<E>(dd.v + e * E, dd2[e]);
           float a0, a1, b0, b1;
-          unpack(mul2(dyp, u), a0, a1);
-          unpack(dd2, b0, b1);
-          add[e] += a0, add[V + e] += b0;
-          if constexpr (E == 2) add[e + 1] += a1, add[V + e + 1] += b1;
+          unpack(mul2(dyp[e], pair_of<E>(raw.u[i].v + e * E)), a0, a1);
+          unpack(dd2[e], b0, b1);
+          add[e * E] += a0, add[V + e * E] += b0;
+          if constexpr (E == 2) add[e * E + 1] += a1, add[V + e * E + 1] += b1;
         }
         *reinterpret_cast<Vec<T, V>*>(p.du + t * p.lddu + d) = du;
         *reinterpret_cast<Vec<T, V>*>(p.ddelta + t * p.ldddelta + d) = dd;

@@ -609,6 +609,90 @@ def test_bad_slots_are_reported(cuda, slots):
             mk.synchronize(BE)
 
 
+def test_columns_outside_the_sequences_are_never_read(cuda):
+    """NaN in front of, between batches' ends and behind the sequences, and in states that no sequence uses."""
+    lens, D, N, W, lead, tail = [37, 0, 50], 40, 16, 4, 5, 9
+    c = scan_case(lens, D, N, 1, lead, tail, True, True, True, True, True, "BFloat16")
+    m = torch.from_numpy(inside(c["spans"], c["T"])).cuda()
+
+    def poison(a):
+        a.storage.view(c["T"], -1)[~m] = float("nan")
+
+    seqs = seqs_of(c["spans"])
+    w, _ = dev(gen(3).standard_normal((W, D)))
+    h0, _ = dev(gen(4).standard_normal((3, W - 1, D)), "BFloat16")
+
+    def everything():
+        saved = mk.selective_scan_saved(c["u"], c["A"], seqs=seqs)
+        y, last = scan_forward(c, saved)
+        g = scan_grad(c, saved)
+        t = "BFloat16"
+        cy, dx, dw = out((c["T"], D), t), out((c["T"], D), t), out((W, D))
+        cl, di = out((3, W - 1, D), t), out((3, W - 1, D), t)
+        mk.causal_conv(cy, c["u"], w, seqs=seqs, init=h0, last=cl)
+        mk.causal_conv_grad(dx, dw, c["dy"], c["u"], w, seqs=seqs, init=h0, dinit=di, dlast=h0)
+        mk.synchronize(BE)
+        return [host(x) for x in [y, last, cy, dx, dw, cl, di] + [x for x in g.values() if x is not None]]
+
+    want = everything()
+    for k in ("u", "delta", "z", "B", "C", "dy"):
+        poison(c[k])
+    for a, b in zip(want, everything()):
+        assert np.isfinite(b).all()
+        np.testing.assert_array_equal(a, b)
+
+
+def test_columns_beyond_two_to_the_31_elements(cuda):
+    """Rows of a matrix of 2.2e9 elements: the last columns against the same columns on their own."""
+    D, T, ld = 64, 2100, 1 << 20
+    parent = mk.MLIRArray(torch.zeros(ld * T, dtype=torch.bfloat16, device="cuda"), dims=(ld, T))
+    x = mk.rows(parent, ld - D + 1, ld)
+    view = parent.storage.view(T, ld)[:, ld - D:]
+    r = gen(12)
+    xs, _ = dev(r.standard_normal((T, D)), "BFloat16")
+    view.copy_(xs.storage.view(T, D))
+    w, _ = dev(r.standard_normal((4, D)))
+    A, _ = dev(-np.exp(r.standard_normal((D, 4))))
+    B, _ = dev(r.standard_normal((T, 4)), "BFloat16")
+    one, _ = dev(np.ones(D))
+    for call in (lambda y, a: mk.causal_conv(y, a, w), lambda y, a: mk.selective_scan(y, a, a, A, B, B, z=a),
+                 lambda y, a: mk.block_norm(y, None, a, one)):
+        far, near = out((T, D), "BFloat16"), out((T, D), "BFloat16")
+        call(far, x)
+        call(near, xs)
+        mk.synchronize(BE)
+        np.testing.assert_array_equal(host(far), host(near))
+
+
+def test_many_short_sequences(cuda):
+    """More sequences than a warp looks over at once, most of them short or empty."""
+    r = gen(13)
+    lens = list(r.integers(0, 4, 1500)) + [70] + list(r.integers(0, 2, 300))
+    c = scan_case([int(n) for n in lens], 16, 4, 1, 1, 2, True, True, True, True, True, "Float32")
+    saved = mk.selective_scan_saved(c["u"], c["A"], seqs=seqs_of(c["spans"]))
+    y, last = scan_forward(c, saved)
+    g = scan_grad(c, saved)
+    w, wv = dev(r.standard_normal((4, 16)))
+    x, xv = c["u"], c["v"]["u"]
+    cy, dx, dw = out((c["T"], 16)), out((c["T"], 16)), out((4, 16))
+    mk.causal_conv(cy, x, w, seqs=seqs_of(c["spans"]))
+    mk.causal_conv_grad(dx, dw, c["dy"], x, w, seqs=seqs_of(c["spans"]))
+    mk.synchronize(BE)
+    m = inside(c["spans"], c["T"])
+    (wy, wl, wg), (my, ml, mg) = scan_ref(c, True), scan_ref(c, True, True)
+    ref.close(host(y)[m], wy[m], my[m], "Float32", k_scan(c))
+    ref.close(host(last), wl, ml, "Float32", k_scan(c))
+    for name in ("u", "delta", "z", "B", "C"):
+        ref.close(host(g[name])[m], wg[name][m], mg[name][m], "Float32", k_scan(c), name)
+    for name in ("A", "D", "bias", "init"):
+        ref.close(host(g[name]), wg[name], mg[name], "Float32", k_scan(c) + c["T"] / 8, name)
+    a = (xv, wv, np.zeros(16), True, c["spans"], None, c["v"]["dy"])
+    want, mag = ref.conv(*a), ref.conv(*a, mag=True)
+    ref.close(host(cy)[m], want[0][m], mag[0][m], "Float32", 64)
+    ref.close(host(dx)[m], want[2][m], mag[2][m], "Float32", 64)
+    ref.close(host(dw), want[3], mag[3], "Float32", 64 + c["T"] / 8)
+
+
 def test_nothing_to_do(cuda):
     """No tokens, no sequences, no batch entries."""
     A, _ = dev(-np.ones((8, 16)))

@@ -18,7 +18,8 @@ using namespace mk::tok;
 
 template <typename T, typename R>
 struct Norm {
-  int64_t D, T_;
+  int D;  // at most 16384
+  int64_t T_;
   float eps, inv_d;
   int act;
   const R *r, *drout;
@@ -98,6 +99,10 @@ struct Column {
 
   // Column t; zeros for what is not there.
   __device__ __forceinline__ void fetch(const Norm<T, R>& p, int64_t t) {
+    const R* pr = p.r + t * p.ldr;
+    const T *ph = p.h + t * p.ldh, *pg = p.gate + t * p.ldgate;
+    const T* pdy = GRAD ? p.dy + t * p.lddy : nullptr;
+    const R* pdro = GRAD ? p.drout + t * p.lddrout : nullptr;
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
 #pragma unroll
@@ -105,16 +110,19 @@ struct Column {
         r[k].v[i] = from_f<R>(0.0f), h[k].v[i] = g[k].v[i] = from_f<T>(0.0f);
         if constexpr (GRAD) dro[k].v[i] = from_f<R>(0.0f), dy[k].v[i] = from_f<T>(0.0f);
       }
-      const int64_t d = ((int64_t)k * blockDim.x + threadIdx.x) * V;
-      const bool on = d < p.D && t < p.T_;
-      load_vec<T, V>(h[k], p.h + t * p.ldh + d, on && p.h);
-      load_vec<R, V>(r[k], p.r + t * p.ldr + d, on);
-      load_vec<T, V>(g[k], p.gate + t * p.ldgate + d, on && p.gate);
-      if constexpr (GRAD) {
-        load_vec<T, V>(dy[k], p.dy + t * p.lddy + d, on && p.dy);
-        load_vec<R, V>(dro[k], p.drout + t * p.lddrout + d, on && p.drout);
-      }
     }
+    // one matrix after the other: whether it is there is asked once, not per vector
+    auto all = [&](auto& to, const auto* from, bool there) {
+      if (!there) return;
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) {
+        const int d = (k * (int)blockDim.x + (int)threadIdx.x) * V;
+        load_vec(to[k], from + d, d < p.D);
+      }
+    };
+    if (t >= p.T_) return;
+    all(h, ph, p.h), all(r, pr, true), all(g, pg, p.gate);
+    if constexpr (GRAD) all(dy, pdy, p.dy), all(dro, pdro, p.drout);
   }
   __device__ __forceinline__ float sum_hh() const;
 };
@@ -135,10 +143,10 @@ __device__ __forceinline__ void put_pair(Vec<X, V> (&r)[ITEMS], int j, F2 x) {
   }
 }
 template <typename X, int V, int ITEMS>
-__device__ __forceinline__ void store_column(X* column, int64_t D, const Vec<X, V> (&r)[ITEMS]) {
+__device__ __forceinline__ void store_column(X* column, int D, const Vec<X, V> (&r)[ITEMS]) {
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const int64_t d = ((int64_t)k * blockDim.x + threadIdx.x) * V;
+    const int d = (k * (int)blockDim.x + (int)threadIdx.x) * V;
     if (d < D) *reinterpret_cast<Vec<X, V>*>(column + d) = r[k];
   }
 }
@@ -156,11 +164,11 @@ __device__ __forceinline__ float Column<T, R, V, ITEMS, GRAD>::sum_hh() const {
 
 // A thread's values of a parameter, ones without it.
 template <int V, int ITEMS>
-__device__ __forceinline__ void param(F2 (&f)[V * ITEMS / 2], const float* p, int64_t D) {
+__device__ __forceinline__ void param(F2 (&f)[V * ITEMS / 2], const float* p, int D) {
   Vec<float, V> r[ITEMS];
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const int d = (k * blockDim.x + threadIdx.x) * V;
+    const int d = (k * (int)blockDim.x + (int)threadIdx.x) * V;
 #pragma unroll
     for (int i = 0; i < V; ++i) r[k].v[i] = 1.0f;
     load_vec<float, V>(r[k], p + d, p && d < D);
@@ -488,23 +496,24 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ahead(Norm<T, R> p) {
   }
 }
 
-// dw, dhw, dscale: the sums over the column walkers, 32 values and 8 ranges of
+// dw, dhw, dscale: the sums over the column walkers, 32 values and 16 ranges of
 // walkers per block.
-__global__ void __launch_bounds__(256) norm_fold(const float* parts, int64_t nparts, int64_t D, float* dw, float* dhw,
-                                                 float* dscale) {
-  __shared__ float sm[8][32];
+constexpr int kFoldRows = 16;
+__global__ void __launch_bounds__(32 * kFoldRows) norm_fold(const float* parts, int64_t nparts, int64_t D, float* dw,
+                                                            float* dhw, float* dscale) {
+  __shared__ float sm[kFoldRows][32];
   const int64_t i = (int64_t)blockIdx.x * 32 + threadIdx.x, n = 3 * D;
   float v = 0.0f;
   if (i < n) {
-#pragma unroll 4
-    for (int64_t k = threadIdx.y; k < nparts; k += 8) v += parts[k * n + i];
+#pragma unroll 8
+    for (int64_t k = threadIdx.y; k < nparts; k += kFoldRows) v += parts[k * n + i];
   }
   sm[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   if (threadIdx.y || i >= n) return;
   v = 0.0f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v += sm[k][threadIdx.x];
+  for (int k = 0; k < kFoldRows; ++k) v += sm[k][threadIdx.x];
   float* out = i < D ? dw : i < 2 * D ? dhw : dscale;
   if (out) out[i % D] = v;
 }
@@ -573,7 +582,7 @@ dim3 block_of(int64_t D, int V, int items) {
 template <typename T, typename R>
 Norm<T, R> params(const mk_norm_args* a) {
   Norm<T, R> p{};
-  p.D = a->D, p.T_ = a->T, p.eps = a->eps, p.inv_d = 1.0f / (float)a->D, p.act = a->act;
+  p.D = (int)a->D, p.T_ = a->T, p.eps = a->eps, p.inv_d = 1.0f / (float)a->D, p.act = a->act;
   p.r = static_cast<const R*>(a->r), p.ldr = a->ldr;
   p.h = static_cast<const T*>(a->h), p.ldh = a->ldh;
   p.gate = static_cast<const T*>(a->gate), p.ldgate = a->ldgate;
@@ -634,7 +643,7 @@ int launch_bwd(const mk_norm_args* a, const BwdPlan& b, cudaStream_t s) {
   const size_t smem = (size_t)3 * V * ITEMS * sizeof(float) * b.block.x * b.block.y;
   MK_TRY(mk::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem));
   if (b.grid) kernel<<<(unsigned)b.grid, b.block, smem, s>>>(p);
-  norm_fold<<<(unsigned)mk::cdiv(3 * a->D, 32), dim3(32, 8), 0, s>>>(p.parts, b.parts, a->D, a->dw, a->dhw, a->dscale);
+  norm_fold<<<(unsigned)mk::cdiv(3 * a->D, 32), dim3(32, kFoldRows), 0, s>>>(p.parts, b.parts, a->D, a->dw, a->dhw, a->dscale);
   return mk::check_launch("mk_block_norm_grad: launch");
 }
 
@@ -646,7 +655,7 @@ int launch_bwd_ahead(const mk_norm_args* a, const BwdPlan& b, cudaStream_t s) {
   const size_t smem = (size_t)(S * (2 * 8 * sizeof(R) / 16 + 3) + 6) * 16 * b.block.x * b.block.y;
   MK_TRY(mk::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem));
   if (b.grid) kernel<<<(unsigned)b.grid, b.block, smem, s>>>(p);
-  norm_fold<<<(unsigned)mk::cdiv(3 * a->D, 32), dim3(32, 8), 0, s>>>(p.parts, b.parts, a->D, a->dw, a->dhw, a->dscale);
+  norm_fold<<<(unsigned)mk::cdiv(3 * a->D, 32), dim3(32, kFoldRows), 0, s>>>(p.parts, b.parts, a->D, a->dw, a->dhw, a->dscale);
   return mk::check_launch("mk_block_norm_grad: launch");
 }
 

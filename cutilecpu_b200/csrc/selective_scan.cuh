@@ -128,7 +128,7 @@ __device__ __forceinline__ Item item_at(const Scan<T>& p, int64_t i) {
   it.hi = sp.hi;
   it.t0 = sp.lo + it.c * p.piece;
   it.t1 = p.piece ? min(sp.hi, it.t0 + p.piece) : sp.hi;
-  it.none = it.c > 0 && it.t0 >= sp.hi;
+  it.none = it.c < 0 || (it.c > 0 && it.t0 >= sp.hi);  // below 0: columns in front of the first sequence
   return it;
 }
 

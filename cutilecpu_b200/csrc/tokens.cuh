@@ -168,7 +168,8 @@ __device__ __forceinline__ int64_t first_piece(const Seqs& q, int64_t s, int64_t
   return seq_offset(q, s) / piece + s;
 }
 
-// The sequence that piece number `i` falls to (the last s with first_piece <= i).
+// The sequence that piece number `i` falls to (the last s with first_piece <= i;
+// the first sequence, if none, when columns in front of it belong to no sequence).
 __device__ __forceinline__ int64_t seq_of_piece(const Seqs& q, int64_t i, int64_t piece) {
   int64_t lo = 0, hi = q.nseq - 1;
   while (lo < hi) {
@@ -261,8 +262,7 @@ constexpr float kDecayBias = 3.0e-8f;
 __device__ __forceinline__ float decay(float dt, float A2) { return ex2(fmaf(dt, A2, kDecayBias)); }
 __device__ __forceinline__ F2 decay2(F2 dt, F2 A2) { return ex2_2(fma2(dt, A2, pack(kDecayBias))); }
 
-// Two neighbouring elements as a pair, and back.
-template <typename T> __device__ __forceinline__ F2 to_f2(const T* p) { return pack(to_f(p[0]), to_f(p[1])); }
+// A pair as two neighbouring elements.
 __device__ __forceinline__ void from_f2(float* p, F2 x) { unpack(x, p[0], p[1]); }
 __device__ __forceinline__ void from_f2(__half* p, F2 x) {
   float a, b;

@@ -642,6 +642,27 @@ def test_columns_outside_the_sequences_are_never_read(cuda):
         np.testing.assert_array_equal(a, b)
 
 
+def test_pieces_behind_columns_of_no_sequence(cuda):
+    """Sequences cut into pieces behind more uncovered columns than a piece has (NaN there): they stay as they were."""
+    c = scan_case([600, 0, 90], 33, 16, 1, 270, 130, True, True, True, True, True, "Float32")
+    m = inside(c["spans"], c["T"])
+    for k in ("u", "delta", "z", "B", "C", "dy"):
+        c[k].storage.view(c["T"], -1)[~torch.from_numpy(m).cuda()] = float("nan")
+    saved = mk.selective_scan_saved(c["u"], c["A"], seqs=seqs_of(c["spans"]))
+    y, last = scan_forward(c, saved)
+    g = scan_grad(c, saved)
+    mk.synchronize(BE)
+    (wy, wl, wg), (my, ml, mg) = scan_ref(c, True), scan_ref(c, True, True)
+    ref.close(host(y)[m], wy[m], my[m], "Float32", k_scan(c))
+    ref.close(host(last), wl, ml, "Float32", k_scan(c))
+    assert (host(y)[~m] == 7.0).all()
+    for name in ("u", "delta", "z", "B", "C"):
+        ref.close(host(g[name])[m], wg[name][m], mg[name][m], "Float32", k_scan(c), name)
+        assert (host(g[name])[~m] == 7.0).all(), name
+    for name in ("A", "D", "bias", "init"):
+        ref.close(host(g[name]), wg[name], mg[name], "Float32", k_scan(c) + c["T"] / 8, name)
+
+
 def test_columns_beyond_two_to_the_31_elements(cuda):
     """Rows of a matrix of 2.2e9 elements: the last columns against the same columns on their own."""
     D, T, ld = 64, 2100, 1 << 20

@@ -236,7 +236,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_fwd(Norm<T, R> p) {
 // sums for w, hw and scale in shared memory, every thread its own channels'
 // (in registers they would leave one block to an SM, and two overlap each
 // other's waits); they go to one part per column walker, added up by norm_fold
-// in a fixed order.
+// in a fixed order.  1027 columns of 1999 channels (f16, single elements): 26 us
+// and 4 us for norm_fold; bound by the waits
+// on its loads and the three reductions of a column (issue slots 48% used).
 template <typename T, typename R, int V, int ITEMS, int THREADS, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS) norm_bwd(Norm<T, R> p) {
   constexpr bool kExact = sizeof(T) == 4;
@@ -330,6 +332,10 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_bwd(Norm<T, R> p) {
 // copies and reads back its own pieces, no barrier), the parameters lie there
 // in the threads' order, and mean(h^2) of the next column is reduced together
 // with the present one's last sum: two reductions per column instead of three.
+// 8192 columns of 4096 channels (bf16, r in Float32): 214 us, 3.5 TB/s, against
+// 270 us by norm_bwd (2048 channels 95 against 125 us, 1024 46 against 60, 512 30
+// against 28).  What is left are waits, on shared memory, shuffles and the two
+// reductions of a column, at four warps per scheduler (issue slots 39% used).
 template <typename T, typename R, int S>
 __global__ void __launch_bounds__(512, 1) norm_bwd_ahead(Norm<T, R> p) {
   constexpr int V = 8, H = V / 2, kR = V * sizeof(R) / 16, kPieces = 2 * kR + 3;  // h, gate, dy, r, drout
@@ -606,7 +612,9 @@ int launch_fwd(const mk_norm_args* a, cudaStream_t s) {
 }
 
 // 16 values per thread; columns of up to 4096 channels take 256 threads at
-// most, so that the registers hold four of them on an SM.
+// most, so that the registers hold four of them on an SM: 8192 x 4096 (bf16, r in
+// Float32) 83 us, 5.7 TB/s, against 116 us with 8 values of 512 threads (2048
+// channels 44 against 49, 1024 and 512 the same).
 template <typename T, typename R>
 int run_fwd(const mk_norm_args* a, cudaStream_t s) {
   constexpr int V = sizeof(T) == 2 ? 8 : 4;

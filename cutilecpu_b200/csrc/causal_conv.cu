@@ -9,6 +9,12 @@
 // their last W - 1 inputs in registers and walks TT tokens, with the next
 // tokens' loads in flight while it computes.  The W - 1 tokens before a tile are
 // read again (they hit L2), which is all that is read twice.
+//
+// bf16, 4 taps, silu, measured on B200: 16384 tokens of 4096 channels forward 55
+// us (4.9 TB/s, 0.75 of a copy; 59 us with the state pool of 7 ragged prompts),
+// 8192 x 4096 forward 29 us (4.6 TB/s), backward 57 us (3.5 TB/s: its
+// registers leave 2.5 to 4 warps to a scheduler, which use half of the issue
+// slots) and 4.3 us for conv_fold; one token of 192 entries of 4099 channels (f32, 3 taps) 5.9 us.
 #include <type_traits>
 
 #include "tokens.cuh"
@@ -471,7 +477,9 @@ bool overlap(const void* a, size_t na, const void* b, size_t nb) {
 }
 
 // Tokens per tile: long tiles read fewer tokens twice, but the launch wants
-// four blocks per SM; short inputs take shorter tiles down to 8 tokens.
+// four blocks per SM; short inputs take shorter tiles down to 8 tokens.  8192 x
+// 4096 forward and backward with tiles of 8, 16, 32, 64, 128 tokens: 175, 126, 102,
+// 92, 97 us; 512 x 2048 with 8, 16, 32, 64: 14.7, 15.7, 21, 30 us.
 int tokens_per_tile(const mk::Device* dev, int64_t T, int64_t dblocks, int most) {
   int tt = most;
   while (tt > 8 && mk::cdiv(T, (int64_t)tt * kRows) * dblocks < 4ll * dev->sms) tt /= 2;

@@ -11,7 +11,9 @@ using namespace mk::scan;
 // bytes per lane and channel, P lanes per channel in memory order.  A thread
 // takes IT channels, so that as many states are in flight and one read of B
 // and C serves them all; with IT == P each of the P lanes also computes what
-// one of those channels needs once (softplus, gate), and passes it round.
+// one of those channels needs once (softplus, gate), and passes it round.  192
+// entries of 4096 channels with 16 states: 21 us, 5.0 TB/s; the copies' rate is
+// not reached because a launch this short spends 3 us starting and ending.
 template <typename T>
 struct Step {
   int64_t D, N, G, Dg, B, nslots, tiles, tpg;  // channel tiles, and of one group
@@ -162,31 +164,45 @@ int check_scan(const char* who, const mk_scan_args* a, bool grad) {
   return check_floats(who, "dinit", a->dinit, false, vec);
 }
 
-// Channels per lane.  Forward: one, two gain nothing.  Backward: two halve what
-// is read from shared memory and reduced over channels, but also the warps, and
-// their registers leave two blocks to an SM; at 1.7 blocks per SM they measured
-// 976 us against 1066 us, so they are taken from 1.5 on.
-int channels_of(const mk_scan_args* a, const mk::Device* dev, bool grad) {
-  if (!grad || a->N > 16) return 1;  // the registers hold no two channels of 8 states
-  const int64_t blocks = a->G * mk::cdiv(a->D / a->G, kWarps * 2 * 32 / lanes_of(a->N)) * a->nseq;
-  return 2 * blocks >= 3 * (int64_t)dev->sms ? 2 : 1;
-}
-
-// Whole sequences while their warps give every scheduler about two; with fewer
-// rows sequences are cut into pieces, as many as would fill the GPU that far.
-// Cutting costs a second pass of exponentials, so it has to win more than 2x.
+// Whole sequences or pieces, and the channels per lane (times: B200, bf16, 16
+// states; `fill`: blocks of whole sequences over the four that an SM holds).
+//
+// Forward, cutting costs a second pass of exponentials: it pays below a third
+// of a fill (1 x 16384 tokens of 640 channels 829 -> 134 us, 3 x 5461 of 2048 at
+// 0.32 396 -> 379 us; 6 x 2730 of 1536 at 0.49 would be 204 -> 300 us).
+// Backward the extra pass is a seventh of the work, and more and shorter blocks
+// even out the end: up to 3/4 of a fill for equal lengths (4 x 2048 of 2048
+// channels 705 -> 502 us, of 4096 at 0.86 926 -> 989 us).  With offsets the
+// lengths are the device's, and one that is long takes the whole sequences'
+// time: up to 3/2 (96, 1000, 3000 and 4096 tokens of 4096 channels 1708 -> 981 us,
+// 4 x 2048 of 6144 at 1.3 1550 -> 1378 us, against the 63 us lost at 0.86).
+// Eight blocks per SM, two rounds, measured best among 4 to 16.
+//
+// Channels per lane, forward: one (two: 262 -> 270 us).  Backward: two halve what
+// is read from shared memory and reduced over channels, but also the warps: 1015
+// -> 926 us for 4 x 2048 tokens of 4096 channels, 827 -> 922 us of 2560.  So two
+// from 1.5 of their blocks per SM on, and in pieces where the blocks that an SM
+// holds (two) get 512 tokens each (4 x 2048 of 2048 455 -> 422 us; 1 x 8192 of
+// 1024, 443 tokens, 235 -> 254 us).
 Plan plan(const mk_scan_args* a, const mk::Device* dev, bool grad) {
   Plan b{};
-  const int64_t Dg = a->D / a->G;
-  b.ch = channels_of(a, dev, grad);
-  const int64_t CB = kWarps * (32 / lanes_of(a->N)) * b.ch;
-  b.tpg = mk::cdiv(Dg, CB);
+  const int64_t Dg = a->D / a->G, sms = dev->sms, CB = kWarps * (32 / lanes_of(a->N));
+  b.rev_tpg = mk::cdiv(Dg, CB);
+  b.rev_tiles = a->G * b.rev_tpg;
+  const int64_t have = b.rev_tiles * a->nseq, twice = a->G * mk::cdiv(Dg, 2 * CB);
+  const bool cut = have > 0 && a->T >= a->nseq * 4 * kTS &&
+                   (grad ? have <= sms * (a->seqs ? 6 : 3) : have * 3 <= 4 * sms);
+  b.ch = 1;
+  if (grad && a->N <= 16) {  // the registers hold no two channels of 8 states
+    const bool enough = cut ? twice * a->T >= 2 * sms * 512 : 2 * twice * a->nseq >= 3 * sms;
+    if (enough) b.ch = 2;
+  }
+  b.tpg = mk::cdiv(Dg, CB * b.ch);
   b.tiles = a->G * b.tpg;
   b.items = a->nseq;
-  const int64_t want = (int64_t)dev->sms * 4, have = b.tiles * a->nseq;
-  if (b.ch == 1 && have > 0 && have * 3 <= want && a->T >= a->nseq * 4 * kTS) {
-    const int64_t pieces = want / b.tiles;  // over all sequences
-    int64_t piece = mk::cdiv(mk::cdiv(a->T, pieces), kTS) * kTS;
+  if (cut) {
+    const int64_t pieces = mk::cdiv(8 * sms, b.tiles);  // over all sequences
+    const int64_t piece = mk::cdiv(mk::cdiv(a->T, pieces), kTS) * kTS;
     b.piece = piece < 2 * kTS ? 2 * kTS : piece;
     b.items = a->T / b.piece + a->nseq;
     b.piece_bytes = align256((size_t)b.items * a->D * a->N * 4) + align256((size_t)b.items * a->D * 4);
@@ -207,7 +223,7 @@ int run_scan(const char* who, const mk_scan_args* a, bool grad, void* stream) {
   if (a->nseq == 0 && !grad) return MK_OK;
   MK_ENTRY_DEVICE(dev);
   const Plan b = plan(a, dev, grad);
-  if (b.tiles * b.items > INT32_MAX) return bad(who, "too many sequences for these channels");
+  if (b.rev_tiles * b.items > INT32_MAX) return bad(who, "too many sequences for these channels");
   if (b.bytes && (!a->workspace || a->workspace_bytes < b.bytes || !elem_aligned(a->workspace, 16)))
     return bad(who, "a 16-byte aligned workspace of " + std::to_string(b.bytes) + " bytes is needed");
   cudaStream_t s = mk::as_stream(stream);
@@ -226,7 +242,8 @@ int workspace(const char* who, const mk_scan_args* a, bool grad, size_t* bytes) 
 
 template <typename T, int P>
 int launch_step(Step<T> p, const mk::Device* dev, cudaStream_t s) {
-  // P channels per thread (up to 8), one where that would leave SMs without a block
+  // P channels per thread (up to 8): at 192 entries of 4096 channels and 16 states 47.6 -> 25.1 us, at 16 entries 6.9
+  // -> 5.3; one where fewer than two blocks per SM would be left (8 entries: 4.5 -> 4.4 us, 1 entry 3.9 -> 3.7)
   constexpr int IT = P <= 8 ? P : 1;
   const int64_t few = p.G * mk::cdiv(p.Dg, IT * (128 / P));
   const bool wide = few * p.B >= 2 * (int64_t)dev->sms;

@@ -642,6 +642,31 @@ def test_columns_outside_the_sequences_are_never_read(cuda):
         np.testing.assert_array_equal(a, b)
 
 
+@pytest.mark.parametrize("N", [16, 7])
+def test_many_channels_in_pieces(cuda, N):
+    """Enough tokens and channels for two channels per lane in pieces; the first and the last group are compared."""
+    D, G = 2048, 32
+    c = scan_case([2600, 0, 2000, 437], D, N, G, 0, 0, True, True, True, True, True, "BFloat16")
+    saved = mk.selective_scan_saved(c["u"], c["A"], seqs=seqs_of(c["spans"]))
+    y, last = scan_forward(c, saved)
+    g = scan_grad(c, saved)
+    mk.synchronize(BE)
+    ch, gr = np.r_[:D // G, D - D // G:D], [0, G - 1]
+    v = c["v"]
+    sub = dict(c, D=2 * (D // G), v={k: v[k][:, ch] for k in ("u", "delta", "z", "dy", "init", "dlast")}
+               | {k: v[k][ch] for k in ("A", "skip", "bias")} | {k: v[k][:, gr] for k in ("B", "C")})
+    (wy, wl, wg), (my, ml, mg) = scan_ref(sub, True), scan_ref(sub, True, True)
+    ref.close(host(y)[:, ch], wy, my, "BFloat16", k_scan(c))
+    ref.close(host(last)[:, ch], wl, ml, "Float32", k_scan(c))
+    for name in ("u", "delta", "z"):
+        ref.close(host(g[name])[:, ch], wg[name], mg[name], "BFloat16", k_scan(c), name)
+    for name in ("B", "C"):
+        ref.close(host(g[name])[:, gr], wg[name], mg[name], "BFloat16", k_scan(c), name)
+    for name in ("A", "D", "bias"):
+        ref.close(host(g[name])[ch], wg[name], mg[name], "Float32", k_scan(c) + c["T"] / 8, name)
+    ref.close(host(g["init"])[:, ch], wg["init"], mg["init"], "Float32", k_scan(c) + c["T"] / 8, "init")
+
+
 def test_pieces_behind_columns_of_no_sequence(cuda):
     """Sequences cut into pieces behind more uncovered columns than a piece has (NaN there): they stay as they were."""
     c = scan_case([600, 0, 90], 33, 16, 1, 270, 130, True, True, True, True, True, "Float32")

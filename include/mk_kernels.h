@@ -2,7 +2,9 @@
  * mk_kernels.h — C ABI of libkernels.so, the B200 (sm_100a) kernel library
  * that replaces the JIT-compiled GPU path of MLIRKernels.jl (gbaraldi/cuTileCPU)
  * for five data-parallel kernels: vadd, mapreduce, gather, histogram and the
- * 16x16 @localmem tiled matmul.
+ * 16x16 @localmem tiled matmul.  Beside them: reductions, scans, maps and
+ * pools, and the operators of state space layers (causal convolution,
+ * selective scan, block norms).
  *
  * Conventions (all entry points):
  *   - Return an int status: MK_OK (0) or a negative MK_ERR_* code. On failure a
@@ -318,9 +320,10 @@ MK_API int mk_peer_trace(unsigned long long* log_dev, int entries);
  * nslots is treated as having none; what a shared slot holds is undefined).
  *
  * None of them allocates: what a call needs is a workspace of the size that
- * the *_workspace function gives, 16-byte aligned, owned by the caller, free
- * for other use once the call's work on the stream is done.  Matrices that are written must not
- * overlap others unless said so below.  Results do not depend on timing
+ * the *_workspace function gives for the same arguments (pointers and leading
+ * dimensions count too), 16-byte aligned, owned by the caller, free for other
+ * use once the call's work on the stream is done.  Matrices that are written
+ * must not overlap others unless said so below.  Results do not depend on timing
  * (no floating-point atomics). */
 #define MK_T_F32  0
 #define MK_T_F16  1
@@ -391,8 +394,8 @@ MK_API int mk_causal_conv_step(const mk_conv_step_args* args, void* stream);
  *   h[n] = exp(dt * A[n,d]) * h[n] + dt * u * B[n,g,t]
  *   y = (sum_n C[n,g,t] * h[n] + Dskip[d] * u) * (z ? z*sigmoid(z) : 1)
  * A is (N, D), states are (N, D, sequence) Float32 (16-byte aligned where 4
- * divides N), B and C have G*N rows (n fastest).  1 <= N <= 64.  h starts at init (or zero); `last` receives the
- * final h and may be `init` itself.  y may be u, delta or z (same ld).
+ * divides N), B and C have G*N rows (n fastest).  1 <= N <= 64.  h starts at
+ * init (or zero); `last` receives the final h and may be `init` itself.  y may be u, delta or z (same ld).
  * `saved`, when not NULL, receives the states at the start of every piece of
  * MK_SCAN_PIECE columns: (N, D, T/MK_SCAN_PIECE + nseq) Float32; the gradient
  * needs it.

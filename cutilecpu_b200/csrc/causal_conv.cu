@@ -462,13 +462,14 @@ int check(const mk_conv_args* a, const char* who) {
   if (a->D < 1 || a->T < 0 || a->nseq < 0 || a->len < 0) return bad(who, "negative size or no channels");
   if (a->D > (1ll << 20) || a->T > INT32_MAX || a->nseq > (1ll << 24))
     return bad(who, "more than 2^20 channels, 2^24 sequences or 2^31 - 1 tokens");
-  if (a->slots && a->nslots < 0) return bad(who, "negative number of slots");
+  MK_TRY(check_slots(who, a->slots, a->nslots, a->nseq));
   MK_TRY(check_floats(who, "w", a->w, true, false));
   return check_floats(who, "bias", a->bias, false, false);
 }
 
 int check_seqs(const mk_conv_args* a, const char* who) {
-  return !a->seqs && a->nseq * a->len != a->T ? bad(who, "nseq * len is not T") : MK_OK;
+  if (a->seqs) return MK_OK;
+  return (a->nseq && a->len > a->T) || a->nseq * a->len != a->T ? bad(who, "nseq * len is not T") : MK_OK;
 }
 
 bool overlap(const void* a, size_t na, const void* b, size_t nb) {
@@ -676,6 +677,7 @@ int step(const mk_conv_step_args* a, void* stream) {
   c.type = a->type, c.width = a->width, c.D = a->D, c.T = a->B, c.w = a->w, c.bias = a->bias;
   c.slots = a->slots, c.nslots = a->nslots;
   MK_TRY(check(&c, who));
+  MK_TRY(check_slots(who, a->slots, a->nslots, a->B));
   const size_t es = type_bytes(a->type);
   MK_TRY(check_matrix(who, "x", a->x, a->D, a->ldx, a->B, es));
   MK_TRY(check_matrix(who, "y", a->y, a->D, a->ldy, a->B, es));

@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(128) scan_step(Step<T> p) {
     y[i] = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      h[i][j] = fmaf(decay(dt_i, A[i][j] * kLog2e), h[i][j], dtu_i * b[j]);
+      h[i][j] = fmaf(decay(dt_i, rate(A[i][j])), h[i][j], dtu_i * b[j]);
       y[i] = fmaf(c[j], h[i][j], y[i]);
     }
     if (live[i]) store4(next + d[i] * N, h[i], n0, N);
@@ -129,7 +129,8 @@ int check_sizes(const char* who, int type, int64_t D, int64_t N, int64_t G, int6
 int check_scan(const char* who, const mk_scan_args* a, bool grad) {
   if (!a) return bad(who, "null arguments");
   MK_TRY(check_sizes(who, a->type, a->D, a->N, a->G, a->T, a->nseq));
-  if (a->len < 0 || (!a->seqs && a->nseq * a->len != a->T)) return bad(who, "nseq * len is not T");
+  if (a->len < 0 || (!a->seqs && ((a->nseq && a->len > a->T) || a->nseq * a->len != a->T)))
+    return bad(who, "nseq * len is not T");
   const size_t es = type_bytes(a->type);
   const bool vec = a->N % 4 == 0;
   MK_TRY(check_matrix(who, "u", a->u, a->D, a->ldu, a->T, es));
@@ -142,7 +143,7 @@ int check_scan(const char* who, const mk_scan_args* a, bool grad) {
   MK_TRY(check_floats(who, "bias", a->bias, false, false));
   MK_TRY(check_floats(who, "init", a->init, false, vec));
   MK_TRY(check_floats(who, "saved", a->saved, grad && a->T > 0, vec));
-  if (a->slots && a->nslots < 0) return bad(who, "negative number of slots");
+  MK_TRY(check_slots(who, a->slots, a->nslots, a->nseq));
   if (!grad) {
     MK_TRY(check_matrix(who, "y", a->y, a->D, a->ldy, a->T, es));
     return check_floats(who, "last", a->last, false, vec);
@@ -290,7 +291,7 @@ int step(const mk_scan_step_args* a, void* stream) {
   MK_TRY(check_floats(who, "bias", a->bias, false, false));
   MK_TRY(check_floats(who, "state", a->state, some, vec));
   MK_TRY(check_floats(who, "next", a->next, some, vec));
-  if (a->slots && a->nslots < 0) return bad(who, "negative number of slots");
+  MK_TRY(check_slots(who, a->slots, a->nslots, a->B));
   if (!some) return MK_OK;
   if (a->B * (mk::cdiv(a->D, 8) + a->G) > INT32_MAX) return bad(who, "batch too large for these channels");
   MK_ENTRY_DEVICE(dev);

@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
   for (int i = 0; i < CH; ++i) {
     load_states<NS>(A2[i], p.A + w.d[i] * p.N, n0, p.N);
 #pragma unroll
-    for (int j = 0; j < H; ++j) A2[i][j] = mul2(A2[i][j], pack(kLog2e, kLog2e)), h[i][j] = pack(0.0f, 0.0f);
+    for (int j = 0; j < H; ++j) A2[i][j] = rate2(A2[i][j]), h[i][j] = pack(0.0f, 0.0f);
     // Pieces: entry 0 of a sequence's workspace is its initial state (read from
     // there by every piece, because `last` may replace it), entry c + 1 the
     // state that piece c leaves when it starts from zero.
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(kThreads) scan_rev(Scan<T> p) {
   for (int i = 0; i < CH; ++i) {
     load_states<NS>(A2[i], p.A + w.d[i] * p.N, n0, p.N);
 #pragma unroll
-    for (int j = 0; j < H; ++j) A2[i][j] = mul2(A2[i][j], pack(kLog2e, kLog2e)), e_[i][j] = pack(0.0f, 0.0f);
+    for (int j = 0; j < H; ++j) A2[i][j] = rate2(A2[i][j]), e_[i][j] = pack(0.0f, 0.0f);
   }
   constexpr bool kExact = sizeof(T) == 4;
   constexpr int E = V > 1 ? 2 : 1, Q = V / E;
@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, CH == 1 && NS <= 4 ? 4 : NS == 2 ? 3
   for (int i = 0; i < CH; ++i) {
     load_states<NS>(A2[i], p.A + w.d[i] * p.N, n0, p.N, m);
 #pragma unroll
-    for (int j = 0; j < H; ++j) A2[i][j] = mul2(A2[i][j], pack(kLog2e, kLog2e)), dA[i][j] = pack(0.0f, 0.0f);
+    for (int j = 0; j < H; ++j) A2[i][j] = rate2(A2[i][j]), dA[i][j] = pack(0.0f, 0.0f);
   }
   // A thread's share of the sums for D and bias: 2 V values of its vectors, summed over the RD lanes of the warp that
   // have the same channels, of which it keeps every RD-th.

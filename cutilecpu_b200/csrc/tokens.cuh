@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cfloat>
+
 #include "mk_common.cuh"
 
 namespace mk {
@@ -203,6 +205,9 @@ __device__ __forceinline__ void check_distinct(const int32_t* slots, int64_t i, 
   if (twice) atomicOr(err, ERRBIT_SLOT);
 }
 
+// Each entry is compared with all before it, which bounds their number.
+constexpr int64_t kMostSlotted = 1 << 20;
+
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLog2eLow = 1.92596299e-8f;  // log2(e) - kLog2e
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -259,6 +264,17 @@ __device__ __forceinline__ float sum2(F2 x) {
 // that up over its memory of hundreds of tokens: the exponent gets it back, in
 // the same instruction.  A step of dt = 0 still gives exactly 1.
 constexpr float kDecayBias = 3.0e-8f;
+// A log2(e) of a pair; an infinite rate as the largest finite one, whose product
+// with a step of 0 is 0 (a state beyond its sequence's end stays).
+__device__ __forceinline__ float rate(float A) {
+  const float x = A * kLog2e;
+  return x < -FLT_MAX ? -FLT_MAX : x;
+}
+__device__ __forceinline__ F2 rate2(F2 A) {
+  float a, b;
+  unpack(A, a, b);
+  return pack(rate(a), rate(b));
+}
 __device__ __forceinline__ float decay(float dt, float A2) { return ex2(fmaf(dt, A2, kDecayBias)); }
 __device__ __forceinline__ F2 decay2(F2 dt, F2 A2) { return ex2_2(fma2(dt, A2, pack(kDecayBias))); }
 
@@ -388,6 +404,12 @@ inline int check_matrix(const char* who, const char* name, const void* p, int64_
   if (ld < rows) return bad(who, std::string(name) + " has a leading dimension below its rows");
   if (!elem_aligned(p, es)) return bad(who, std::string(name) + " is not element-aligned");
   return MK_OK;
+}
+
+inline int check_slots(const char* who, const int32_t* slots, int64_t nslots, int64_t entries) {
+  if (!slots) return MK_OK;
+  if (nslots < 0) return bad(who, "negative number of slots");
+  return entries > kMostSlotted ? bad(who, "more than 2^20 entries with slots") : MK_OK;
 }
 
 // Float32 parameters and states; `vec`: read as 16-byte vectors.

@@ -318,6 +318,7 @@ MK_API int mk_peer_trace(unsigned long long* log_dev, int entries);
  * padding: neither its y nor a state is written).  A slot above nslots, or one
  * that two entries share, sets the error word (an entry whose slot is above
  * nslots is treated as having none; what a shared slot holds is undefined).
+ * At most 2^20 entries with slots.
  *
  * None of them allocates: what a call needs is a workspace of the size that
  * the *_workspace function gives for the same arguments (pointers and leading

@@ -379,6 +379,26 @@ def test_scan_long_memory_and_extreme_steps(cuda):
     ref.close(host(y), ref.scan(*a)[0], ref.scan(*a, mag=True)[0], "Float32", 8 * (T + 24))
 
 
+def test_scan_infinite_rate(cuda):
+    """A state that forgets at once (A = -inf): nothing but the last token is in it, at every length of a tile's rest."""
+    r = gen(15)
+    for T in (1, 3, 8, 33, 700):
+        u, uv = dev(r.standard_normal((T, 4)))
+        dl, dv = dev(r.standard_normal((T, 4)))
+        Av = -np.exp(r.standard_normal((4, 6)))
+        Av[:, ::2] = -np.inf
+        A, Av = dev(Av)
+        B, Bv = dev(r.standard_normal((T, 1, 6)))
+        y, last, h0 = out((T, 4)), out((1, 4, 6)), r.standard_normal((1, 4, 6))
+        init, h0 = dev(h0)
+        mk.selective_scan(y, u, dl, A, B, B, init=init, last=last)
+        mk.synchronize(BE)
+        a = (uv, dv, Av, Bv, Bv, np.zeros(4), None, np.zeros(4), True, [(0, T)], h0)
+        (wy, wl), (my, ml) = ref.scan(*a), ref.scan(*a, mag=True)
+        ref.close(host(y), wy, my, "Float32", 8 * (T + 24))
+        ref.close(host(last), wl, ml, "Float32", 8 * (T + 24))
+
+
 # ---- norms -----------------------------------------------------------------------------
 
 NORM = [(1, 1), (3, 7), (5, 64), (2, 100), (33, 256), (3, 1000), (4, 1030), (2, 4096), (3, 4100), (1, 8200), (2, 16384),
@@ -436,6 +456,14 @@ def test_norm(cuda, T, D, eltype, rtype):
             token = name in ("r", "h", "gate")
             ref.close(host(x), ww, top * (1 + np.abs(Rv).max()), rtype if name == "r" else eltype if token else "Float32",
                       (64 + D / 64) * (1 if token else 1 + T / 8), (act, "d" + name))
+
+
+@pytest.mark.parametrize("eltype,rtype", [("Float32", "Float32"), ("BFloat16", "Float32"), ("Float16", "Float16")])
+@pytest.mark.parametrize("T,D", [(6001, 24), (3001, 72), (1500, 520), (700, 2048), (500, 4096), (900, 1001),
+                                 (301, 4104)])
+def test_norm_many_columns(cuda, T, D, eltype, rtype):
+    """More columns than walk at once."""
+    test_norm(cuda, T, D, eltype, rtype)
 
 
 def test_norm_in_place(cuda):

@@ -60,6 +60,8 @@ CASES = [
     ("mk_causal_conv", conv(D=0), "no channels"),
     ("mk_causal_conv", conv(T=-1), "negative"),
     ("mk_causal_conv", conv(len=15), "nseq \\* len"),
+    ("mk_causal_conv", conv(T=0, nseq=4, len=1 << 62), "nseq \\* len"),  # the product passes 64 bits
+    ("mk_causal_conv", conv(slots=P, nslots=4, seqs=P, nseq=(1 << 20) + 1), "2\\^20 entries"),
     ("mk_causal_conv", conv(x=None), "x is null"),
     ("mk_causal_conv", conv(ldx=7), "leading dimension"),
     ("mk_causal_conv", conv(x=P + 1), "element-aligned"),
@@ -71,6 +73,10 @@ CASES = [
     ("mk_causal_conv_grad", conv(dw=None), "dw is null"),
     ("mk_causal_conv_grad", conv(slots=P), "slots are for serving"),
     ("mk_causal_conv_step", _lib.ConvStepArgs(type=0, width=4, D=4, B=1, x=P, ldx=4, y=P, ldy=4, w=P, next=P), "state"),
+    ("mk_causal_conv_step", _lib.ConvStepArgs(type=0, width=4, D=4, B=(1 << 20) + 1, x=P, ldx=4, y=P, ldy=4, w=P, next=P,
+                                              state=P, slots=P, nslots=4), "2\\^20 entries"),
+    ("mk_selective_scan", scan(T=0, nseq=4, len=1 << 62), "nseq \\* len"),
+    ("mk_selective_scan", scan(slots=P, nslots=4, seqs=P, nseq=(1 << 20) + 1), "2\\^20 entries"),
     ("mk_selective_scan", scan(N=0), "1 to 64 states"),
     ("mk_selective_scan", scan(N=65), "1 to 64 states"),
     ("mk_selective_scan", scan(G=3), "groups"),

@@ -184,7 +184,8 @@ int check_scan(const char* who, const mk_scan_args* a, bool grad) {
 // -> 926 us for 4 x 2048 tokens of 4096 channels, 827 -> 922 us of 2560.  So two
 // from 1.5 of their blocks per SM on, and in pieces where the blocks that an SM
 // holds (two) get 512 tokens each (4 x 2048 of 2048 455 -> 422 us; 1 x 8192 of
-// 1024, 443 tokens, 235 -> 254 us).
+// 1024, 443 tokens, 235 -> 254 us).  Single elements take registers that two
+// channels need (4 x 2048 x 4095 1273 -> 1302 us): one.
 Plan plan(const mk_scan_args* a, const mk::Device* dev, bool grad) {
   Plan b{};
   const int64_t Dg = a->D / a->G, sms = dev->sms, CB = kWarps * (32 / lanes_of(a->N));
@@ -194,7 +195,7 @@ Plan plan(const mk_scan_args* a, const mk::Device* dev, bool grad) {
   const bool cut = have > 0 && a->T >= a->nseq * 4 * kTS &&
                    (grad ? have <= sms * (a->seqs ? 6 : 3) : have * 3 <= 4 * sms);
   b.ch = 1;
-  if (grad && a->N <= 16) {  // the registers hold no two channels of 8 states
+  if (grad && a->N <= 16 && all_vec(a, true)) {  // the registers hold no two channels of 8 states
     const bool enough = cut ? twice * a->T >= 2 * sms * 512 : 2 * twice * a->nseq >= 3 * sms;
     if (enough) b.ch = 2;
   }

@@ -298,12 +298,24 @@ __device__ __forceinline__ Cell get_cell(const float2* cell) {
     return {pack(cell->x, 0.0f), pack(cell->y, 0.0f)};
   }
 }
-template <bool EXACT, int E>
-__device__ __forceinline__ F2 softplus_pair(F2 x) {
-  if constexpr (E == 2) return softplus2<EXACT>(x);
-  float a, b;
-  unpack(x, a, b);
-  return pack(softplus<EXACT>(a), 0.0f);
+// softplus of a thread's values; single elements are taken two at a time.
+template <bool EXACT, int E, int NV, int Q>
+__device__ __forceinline__ void softplus_all(F2 (&x)[NV][Q]) {
+  if constexpr (E == 2 || NV % 2) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < Q; ++e) x[i][e] = softplus2<EXACT>(x[i][e]);
+  } else {
+    static_assert(Q == 1, "one element");
+#pragma unroll
+    for (int i = 0; i < NV; i += 2) {
+      float a, b, none;
+      unpack(x[i][0], a, none), unpack(x[i + 1][0], b, none);
+      unpack(softplus2<EXACT>(pack(a, b)), a, b);
+      x[i][0] = pack(a, 0.0f), x[i + 1][0] = pack(b, 0.0f);
+    }
+  }
 }
 template <bool EXACT, int E>
 __device__ __forceinline__ F2 sigmoid_pair(F2 x) {
@@ -430,12 +442,7 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
       for (int i = 0; i < S::NV; ++i)
 #pragma unroll
         for (int e = 0; e < Q; ++e) dt[i][e] = add2(pair_of<E>(cur.delta[i].v + e * E), bias[e]);
-      if (p.softplus) {
-#pragma unroll
-        for (int i = 0; i < S::NV; ++i)
-#pragma unroll
-          for (int e = 0; e < Q; ++e) dt[i][e] = softplus_pair<kExact, E>(dt[i][e]);
-      }
+      if (p.softplus) softplus_all<kExact, E>(dt);
 #pragma unroll
       for (int i = 0; i < S::NV; ++i) {
         const bool in = tt + S::row(i) < it.t1 && S::col() < w.left;  // no token: the state stays
@@ -613,12 +620,7 @@ __global__ void __launch_bounds__(kThreads) scan_rev(Scan<T> p) {
           dt[i][e] = add2(pair_of<E>(cur.delta[i].v + e * E), bias[e]);
           dyp[i][e] = pair_of<E>(cur.u[i].v + e * E);
         }
-      if (p.softplus) {
-#pragma unroll
-        for (int i = 0; i < S::NV; ++i)
-#pragma unroll
-          for (int e = 0; e < Q; ++e) dt[i][e] = softplus_pair<kExact, E>(dt[i][e]);
-      }
+      if (p.softplus) softplus_all<kExact, E>(dt);
       if (p.z) {
 #pragma unroll
         for (int i = 0; i < S::NV; ++i)
@@ -889,12 +891,7 @@ __global__ void __launch_bounds__(kThreads, CH == 1 && NS <= 4 ? 4 : NS == 2 ? 3
             dt[i][e] = add2(pair_of<E>(raw.delta[i].v + e * E), par_pair(0, S::col() + e * E));
             dyp[i][e] = pair_of<E>(raw.dy[i].v + e * E);
           }
-        if (p.softplus) {
-#pragma unroll
-          for (int i = 0; i < S::NV; ++i)
-#pragma unroll
-            for (int e = 0; e < Q; ++e) dt[i][e] = softplus_pair<kExact, E>(dt[i][e]);
-        }
+        if (p.softplus) softplus_all<kExact, E>(dt);
         if (p.z) {
 #pragma unroll
           for (int i = 0; i < S::NV; ++i)
@@ -1239,7 +1236,7 @@ int run_vec(const mk_scan_args* a, const mk::Device* dev, const Plan& b, bool gr
   const bool vec = all_vec(a, grad);
   if (!grad) return vec ? run_fwd<T, NS, P, true>(a, dev, b, s) : run_fwd<T, NS, P, false>(a, dev, b, s);
   if constexpr (NS <= 4) {
-    if (b.ch == 2) return vec ? run_bwd<T, NS, P, 2, true>(a, dev, b, s) : run_bwd<T, NS, P, 2, false>(a, dev, b, s);
+    if (b.ch == 2) return run_bwd<T, NS, P, 2, true>(a, dev, b, s);
   }
   return vec ? run_bwd<T, NS, P, 1, true>(a, dev, b, s) : run_bwd<T, NS, P, 1, false>(a, dev, b, s);
 }

@@ -253,12 +253,21 @@ struct Spread {
   static constexpr int kPerRow = CB / V;
   static constexpr int kCount = kTS * kPerRow;
   static constexpr int NV = (kCount + kThreads - 1) / kThreads;
+  static constexpr int kRows = kThreads / kPerRow;  // rows from a thread's vector to its next
   static __device__ __forceinline__ bool has(int i) {
     return kCount % kThreads == 0 || i * kThreads + (int)threadIdx.x < kCount;
   }
   static __device__ __forceinline__ int row(int i) { return (i * kThreads + threadIdx.x) / kPerRow; }
   static __device__ __forceinline__ int col() { return threadIdx.x % kPerRow * V; }  // the same for every i
 };
+
+// A thread's vectors of a tile from its first one's address on, of the rows below `rows`.
+template <typename S, typename T, int V, int NV>
+__device__ __forceinline__ void fetch_rows(Vec<T, V> (&r)[NV], const T* at, int64_t ld, int rows) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i, at += S::kRows * ld)
+    load_if(r[i], reinterpret_cast<const Vec<T, V>*>(at), S::has(i) && S::row(i) < rows);
+}
 
 template <int E, typename T>
 __device__ __forceinline__ F2 pair_of(const T* p) {
@@ -369,14 +378,11 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
 
   RawFwd<T, V, S::NV> cur, nxt;
   auto load_raw = [&](RawFwd<T, V, S::NV>& r, int64_t tt) {
-#pragma unroll
-    for (int i = 0; i < S::NV; ++i) {
-      const int64_t t = tt + S::row(i), d = w.base + S::col();
-      const bool on = S::has(i) && t < it.t1 && S::col() < w.left;
-      load_if(r.u[i], reinterpret_cast<const Vec<T, V>*>(p.u + t * p.ldu + d), on);
-      load_if(r.delta[i], reinterpret_cast<const Vec<T, V>*>(p.delta + t * p.lddelta + d), on);
-      load_if(r.z[i], reinterpret_cast<const Vec<T, V>*>(p.z + t * p.ldz + d), on && FULL && p.z);
-    }
+    const int64_t t = tt + S::row(0), d = w.base + S::col();
+    const int rows = S::col() < w.left ? (int)min(it.t1 - tt, (int64_t)kTS) : 0;
+    fetch_rows<S>(r.u, p.u + t * p.ldu + d, p.ldu, rows);
+    fetch_rows<S>(r.delta, p.delta + t * p.lddelta + d, p.lddelta, rows);
+    fetch_rows<S>(r.z, p.z + t * p.ldz + d, p.ldz, FULL && p.z ? rows : 0);
   };
   Fetched<NP, T> fB, fC;
   auto fetch = [&](int64_t tt) {
@@ -437,6 +443,7 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
   for (int64_t tt = it.t0; tt < it.t1; tt += kTS) {
     {
       // one step for all values at a time: a branch per value would keep them from overlapping
+      const int rows = S::col() < w.left ? (int)min(it.t1 - tt, (int64_t)kTS) : 0;
       F2 dt[S::NV][Q];
 #pragma unroll
       for (int i = 0; i < S::NV; ++i)
@@ -445,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
       if (p.softplus) softplus_all<kExact, E>(dt);
 #pragma unroll
       for (int i = 0; i < S::NV; ++i) {
-        const bool in = tt + S::row(i) < it.t1 && S::col() < w.left;  // no token: the state stays
+        const bool in = S::row(i) < rows;  // no token: the state stays
 #pragma unroll
         for (int e = 0; e < Q; ++e)
           put_cell<E>(cells + cell2<CB>(S::row(i), S::col() + e * E), dt[i][e],
@@ -521,10 +528,11 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
     }
     __syncthreads();
     if constexpr (FULL) {
+      T* to = p.y + (tt + S::row(0)) * p.ldy + w.base + S::col();
+      const int rows = S::col() < w.left ? (int)min(it.t1 - tt, (int64_t)kTS) : 0;
 #pragma unroll
-      for (int i = 0; i < S::NV; ++i) {
-        const int64_t t = tt + S::row(i);
-        if (!S::has(i) || t >= it.t1 || S::col() >= w.left) continue;
+      for (int i = 0; i < S::NV; ++i, to += S::kRows * p.ldy) {
+        if (!S::has(i) || S::row(i) >= rows) continue;
         F2 y[Q];
 #pragma unroll
         for (int e = 0; e < Q; ++e)
@@ -540,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
         Vec<T, V> out;
 #pragma unroll
         for (int e = 0; e < Q; ++e) out_pair<E>(out.v + e * E, y[e]);
-        *reinterpret_cast<Vec<T, V>*>(p.y + t * p.ldy + w.base + S::col()) = out;
+        *reinterpret_cast<Vec<T, V>*>(to) = out;
       }
     }
     cur = nxt;
@@ -577,14 +585,11 @@ __global__ void __launch_bounds__(kThreads) scan_rev(Scan<T> p) {
   const int64_t n0 = w.p * NS;
   RawFwd<T, V, S::NV> cur, nxt;  // u: dy
   auto load_raw = [&](RawFwd<T, V, S::NV>& r, int64_t tt) {
-#pragma unroll
-    for (int i = 0; i < S::NV; ++i) {
-      const int64_t t = tt + S::row(i), d = w.base + S::col();
-      const bool on = S::has(i) && t < it.t1 && S::col() < w.left;
-      load_if(r.u[i], reinterpret_cast<const Vec<T, V>*>(p.dy + t * p.lddy + d), on);
-      load_if(r.delta[i], reinterpret_cast<const Vec<T, V>*>(p.delta + t * p.lddelta + d), on);
-      load_if(r.z[i], reinterpret_cast<const Vec<T, V>*>(p.z + t * p.ldz + d), on && p.z);
-    }
+    const int64_t t = tt + S::row(0), d = w.base + S::col();
+    const int rows = S::col() < w.left ? (int)min(it.t1 - tt, (int64_t)kTS) : 0;
+    fetch_rows<S>(r.u, p.dy + t * p.lddy + d, p.lddy, rows);
+    fetch_rows<S>(r.delta, p.delta + t * p.lddelta + d, p.lddelta, rows);
+    fetch_rows<S>(r.z, p.z + t * p.ldz + d, p.ldz, p.z ? rows : 0);
   };
   Fetched<NP, T> fC;
   const int64_t tiles = (it.t1 - it.t0 + kTS - 1) / kTS;
@@ -612,6 +617,7 @@ __global__ void __launch_bounds__(kThreads) scan_rev(Scan<T> p) {
   float sum_dt[CH] = {};
   for (; tt >= it.t0; tt -= kTS) {
     {
+      const int rows = S::col() < w.left ? (int)min(it.t1 - tt, (int64_t)kTS) : 0;
       F2 dt[S::NV][Q], dyp[S::NV][Q];
 #pragma unroll
       for (int i = 0; i < S::NV; ++i)
@@ -632,7 +638,7 @@ __global__ void __launch_bounds__(kThreads) scan_rev(Scan<T> p) {
       }
 #pragma unroll
       for (int i = 0; i < S::NV; ++i) {
-        const bool in = tt + S::row(i) < it.t1 && S::col() < w.left;
+        const bool in = S::row(i) < rows;
 #pragma unroll
         for (int e = 0; e < Q; ++e)
           put_cell<E>(cells + cell2<CB>(S::row(i), S::col() + e * E), dt[i][e], dyp[i][e], in, S::has(i));
@@ -807,15 +813,12 @@ __global__ void __launch_bounds__(kThreads, CH == 1 && NS <= 4 ? 4 : NS == 2 ? 3
     part_at[x] = p.parts + ((which * p.tpg + w.tg) * p.q.T + k) * GN + w.g * p.N + n;
   }
   auto load_raw = [&](RawBwd<T, V, S::NV>& r, int64_t tc, int64_t te) {
-#pragma unroll
-    for (int i = 0; i < S::NV; ++i) {
-      const int64_t t = tc + S::row(i), d = w.base + S::col();
-      const bool on = S::has(i) && t < te && S::col() < w.left;
-      load_if(r.u[i], reinterpret_cast<const Vec<T, V>*>(p.u + t * p.ldu + d), on);
-      load_if(r.delta[i], reinterpret_cast<const Vec<T, V>*>(p.delta + t * p.lddelta + d), on);
-      load_if(r.dy[i], reinterpret_cast<const Vec<T, V>*>(p.dy + t * p.lddy + d), on);
-      load_if(r.z[i], reinterpret_cast<const Vec<T, V>*>(p.z + t * p.ldz + d), on && p.z);
-    }
+    const int64_t t = tc + S::row(0), d = w.base + S::col();
+    const int rows = S::col() < w.left ? (int)(te - tc) : 0;
+    fetch_rows<S>(r.u, p.u + t * p.ldu + d, p.ldu, rows);
+    fetch_rows<S>(r.delta, p.delta + t * p.lddelta + d, p.lddelta, rows);
+    fetch_rows<S>(r.dy, p.dy + t * p.lddy + d, p.lddy, rows);
+    fetch_rows<S>(r.z, p.z + t * p.ldz + d, p.ldz, p.z ? rows : 0);
   };
 
   for (int64_t item = item0; item < p.items; item += p.grid_items) {
@@ -860,6 +863,7 @@ __global__ void __launch_bounds__(kThreads, CH == 1 && NS <= 4 ? 4 : NS == 2 ? 3
     for (int64_t ch = last_tile; ch >= 0; --ch) {
       const int64_t tc = it.t0 + ch * kTS, te = min(it.t1, tc + kTS);
       const int nsub = (int)((te - tc + K - 1) / K);
+      const int rows = S::col() < w.left ? (int)(te - tc) : 0;  // of this thread's vectors
       F2 dAc[CH][H];  // the tile's sum, so that long sums stay exact
 #pragma unroll
       for (int i = 0; i < CH; ++i)
@@ -903,7 +907,7 @@ __global__ void __launch_bounds__(kThreads, CH == 1 && NS <= 4 ? 4 : NS == 2 ? 3
         }
 #pragma unroll
         for (int i = 0; i < S::NV; ++i) {
-          const bool in = tc + S::row(i) < te && S::col() < w.left;
+          const bool in = S::row(i) < rows;
 #pragma unroll
           for (int e = 0; e < Q; ++e) {
             const int c = cell2<CB>(S::row(i), S::col() + e * E);
@@ -1020,10 +1024,12 @@ __global__ void __launch_bounds__(kThreads, CH == 1 && NS <= 4 ? 4 : NS == 2 ? 3
         for (int j = 0; j < H; ++j) dA[i][j] = add2(dA[i][j], dAc[i][j]);
       if (VEC && ch > 0) ask(ch - 1);
       float add[2 * V] = {};
+      const int64_t t = tc + S::row(0), d = w.base + S::col();
+      T *to_u = p.du + t * p.lddu + d, *to_d = p.ddelta + t * p.ldddelta + d, *to_z = p.dz + t * p.lddz + d;
 #pragma unroll
-      for (int i = 0; i < S::NV; ++i) {
-        const int64_t t = tc + S::row(i), d = w.base + S::col();
-        if (!S::has(i) || t >= te || S::col() >= w.left) continue;
+      for (int i = 0; i < S::NV;
+           ++i, to_u += S::kRows * p.lddu, to_d += S::kRows * p.ldddelta, to_z += S::kRows * p.lddz) {
+        if (!S::has(i) || S::row(i) >= rows) continue;
         Vec<T, V> du, dd, dz;
         F2 dyp[Q];
         Cell x[Q], y[Q];
@@ -1066,9 +1072,9 @@ __global__ void __launch_bounds__(kThreads, CH == 1 && NS <= 4 ? 4 : NS == 2 ? 3
           add[e * E] += a0, add[V + e * E] += b0;
           if constexpr (E == 2) add[e * E + 1] += a1, add[V + e * E + 1] += b1;
         }
-        *reinterpret_cast<Vec<T, V>*>(p.du + t * p.lddu + d) = du;
-        *reinterpret_cast<Vec<T, V>*>(p.ddelta + t * p.ldddelta + d) = dd;
-        if (p.z) *reinterpret_cast<Vec<T, V>*>(p.dz + t * p.lddz + d) = dz;
+        *reinterpret_cast<Vec<T, V>*>(to_u) = du;
+        *reinterpret_cast<Vec<T, V>*>(to_d) = dd;
+        if (p.z) *reinterpret_cast<Vec<T, V>*>(to_z) = dz;
       }
       float more[ND];
       reduce_scatter<2 * V, RD, S::kPerRow>(add, (threadIdx.x & 31) / S::kPerRow, more);

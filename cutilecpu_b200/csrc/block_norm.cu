@@ -614,16 +614,24 @@ int launch_fwd(const mk_norm_args* a, cudaStream_t s) {
 // 16 values per thread; columns of up to 4096 channels take 256 threads at
 // most, so that the registers hold four of them on an SM: 8192 x 4096 (bf16, r in
 // Float32) 83 us, 5.7 TB/s, against 116 us with 8 values of 512 threads (2048
-// channels 44 against 49, 1024 and 512 the same).
+// channels 44 against 49, 1024 and 512 the same).  Single elements take more
+// registers: 8 values per thread (8192 x 4095 Float32 195 -> 166 us, 1023 bf16 40 ->
+// 38), but for the widest of 16 bits (4095 bf16 162 -> 151 us with 16).
 template <typename T, typename R>
 int run_fwd(const mk_norm_args* a, cudaStream_t s) {
   constexpr int V = sizeof(T) == 2 ? 8 : 4;
   if (all_vec(a, V, false))
     return a->D <= 4096 ? launch_fwd<T, R, V, 16 / V, 256, 4>(a, s) : launch_fwd<T, R, V, 16 / V, 1024, 1>(a, s);
-  return a->D <= 4096 ? launch_fwd<T, R, 1, 16, 256, 3>(a, s) : launch_fwd<T, R, 1, 16, 1024, 1>(a, s);
+  if (a->D > 4096) return launch_fwd<T, R, 1, 16, 1024, 1>(a, s);
+  if constexpr (sizeof(T) == 2) {
+    if (a->D > 2048) return launch_fwd<T, R, 1, 16, 256, 3>(a, s);
+  }
+  return launch_fwd<T, R, 1, 8, 512, 2>(a, s);
 }
 
-// Values per thread: 8, and 16 of the widest columns.
+// Values per thread: 8, and 16 of columns beyond 4096 channels; up to 8192 of
+// them that is 512 threads, which have registers for it (4096 x 8192 bf16 630 -> 305
+// us against code for 1024, 5120 channels 458 -> 219).  Wider ones spill.
 struct BwdPlan {
   int V, items;
   dim3 block;
@@ -673,6 +681,8 @@ int run_bwd(const mk_norm_args* a, const BwdPlan& b, cudaStream_t s) {
   if constexpr (V == 8) {
     if (b.V == 8 && a->D <= 4096) return launch_bwd_ahead<T, R>(a, b, s);
   }
+  if (a->D > 4096 && a->D <= 8192)
+    return b.V == V ? launch_bwd<T, R, V, 16 / V, 512, 1>(a, b, s) : launch_bwd<T, R, 1, 16, 512, 1>(a, b, s);
   if (a->D > 4096)
     return b.V == V ? launch_bwd<T, R, V, 16 / V, 1024, 1>(a, b, s) : launch_bwd<T, R, 1, 16, 1024, 1>(a, b, s);
   if constexpr (V == 4) {

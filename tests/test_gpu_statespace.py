@@ -460,7 +460,7 @@ def test_norm(cuda, T, D, eltype, rtype):
 
 @pytest.mark.parametrize("eltype,rtype", [("Float32", "Float32"), ("BFloat16", "Float32"), ("Float16", "Float16")])
 @pytest.mark.parametrize("T,D", [(6001, 24), (3001, 72), (1500, 520), (700, 2048), (500, 4096), (900, 1001),
-                                 (301, 4104)])
+                                 (301, 4104), (300, 8184), (160, 6001)])
 def test_norm_many_columns(cuda, T, D, eltype, rtype):
     """More columns than walk at once."""
     test_norm(cuda, T, D, eltype, rtype)

@@ -173,17 +173,17 @@ int check_scan(const char* who, const mk_scan_args* a, bool grad) {
 // 0.32 396 -> 379 us; 6 x 2730 of 1536 at 0.49 would be 204 -> 300 us).
 // Backward the extra pass is a seventh of the work, and more and shorter blocks
 // even out the end: up to 3/4 of a fill for equal lengths (4 x 2048 of 2048
-// channels 705 -> 502 us, of 4096 at 0.86 926 -> 989 us).  With offsets the
+// channels 670 -> 499 us, of 4096 at 0.86 916 -> 978 us).  With offsets the
 // lengths are the device's, and one that is long takes the whole sequences'
-// time: up to 3/2 (96, 1000, 3000 and 4096 tokens of 4096 channels 1708 -> 981 us,
-// 4 x 2048 of 6144 at 1.3 1550 -> 1378 us, against the 63 us lost at 0.86).
+// time: up to 3/2 (96, 1000, 3000 and 4096 tokens of 4096 channels 1659 -> 974 us,
+// 4 x 2048 of 6144 at 1.3 1548 -> 1365 us, against the 62 us lost at 0.86).
 // Eight blocks per SM, two rounds, measured best among 4 to 16.
 //
 // Channels per lane, forward: one (two: 262 -> 270 us).  Backward: two halve what
-// is read from shared memory and reduced over channels, but also the warps: 1015
-// -> 926 us for 4 x 2048 tokens of 4096 channels, 827 -> 922 us of 2560.  So two
+// is read from shared memory and reduced over channels, but also the warps: 1017
+// -> 916 us for 4 x 2048 tokens of 4096 channels, 827 -> 922 us of 2560.  So two
 // from 1.5 of their blocks per SM on, and in pieces where the blocks that an SM
-// holds (two) get 512 tokens each (4 x 2048 of 2048 455 -> 422 us; 1 x 8192 of
+// holds (two) get 512 tokens each (4 x 2048 of 2048 457 -> 417 us; 1 x 8192 of
 // 1024, 443 tokens, 235 -> 254 us).  Single elements take registers that two
 // channels need (4 x 2048 x 4095 1273 -> 1302 us): one.
 Plan plan(const mk_scan_args* a, const mk::Device* dev, bool grad) {

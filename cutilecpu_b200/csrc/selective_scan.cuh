@@ -694,11 +694,11 @@ __global__ void __launch_bounds__(kThreads) scan_rev(Scan<T> p) {
 // here lane c holds its states in the order i ^ (c % M) (B and C are staged in
 // M such orders), so what it keeps is always its first registers.
 //
-// 4 x 2048 tokens of 4096 channels, 16 states (bf16): 837 us in pieces, 915 us
+// 4 x 2048 tokens of 4096 channels, 16 states (bf16): 837 us in pieces, 916 us
 // whole; its two exponentials per state and token take 230 us.  What bounds it is
 // latency: 255 registers leave two blocks to an SM, two warps to a scheduler,
 // whose dependent steps (decay, state, gradient) and shuffles leave half of the
-// issue slots empty.  One channel per lane and four blocks per SM measured 1015
+// issue slots empty.  One channel per lane and four blocks per SM measured 1017
 // us, 2 states on each of 8 lanes 1056.
 template <int NS, int P, int CH, int V>
 struct BwdSmem {

@@ -295,14 +295,15 @@ __device__ __forceinline__ void from_f2(__nv_bfloat16* p, F2 x) {
 
 // e^x for the elementwise functions.  The rounding of x log2(e) costs |x| 2^-24
 // of the result, which is below what 16-bit inputs bring; Float32 inputs get
-// the product's rounding error back (EXACT).
+// the product's rounding error back (EXACT) where e^x is finite: multiplied into
+// an infinite one (from 2^128 on) the correction would make it NaN.
 template <bool EXACT>
 __device__ __forceinline__ float exp_of(float x) {
   const float t = x * kLog2e;
   const float e = ex2(t);
   if constexpr (!EXACT) return e;
   const float r = fmaf(x, kLog2eLow, fmaf(x, kLog2e, -t));
-  return fabsf(t) < 150.0f ? fmaf(e, r * kLn2, e) : e;
+  return fabsf(t) < 128.0f ? fmaf(e, r * kLn2, e) : e;
 }
 __device__ __forceinline__ float rcp(float x) {
   float y;

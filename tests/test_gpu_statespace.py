@@ -798,3 +798,113 @@ def test_half_types_of_arrays(cuda):
     p = mk.pool_allocate("BFloat16", (2, 3))
     mk.copyto(BE, p, np.arange(6, dtype=np.float32).reshape(2, 3))
     np.testing.assert_array_equal(mk.Array(p), np.arange(6, dtype=np.float32).reshape(2, 3))
+
+
+# ---- far gates, rates and offsets ------------------------------------------------------------
+
+# A sigmoid below the smallest normal number counts as zero: 2^-126, times a gate of at most 110 and factors below
+# 1e5, is less than this.
+FLUSH = 1e-30
+
+
+@pytest.fixture
+def far_sig(monkeypatch):
+    """The sigmoid with full relative precision far below zero, where 1 + tanh(x / 2) has none left."""
+    def sig(x):
+        e = np.exp(-np.abs(x))
+        return np.where(x < 0, e, 1.0) / (1.0 + e)
+    monkeypatch.setattr(ref, "sig", sig)
+
+
+def near(got, want, mag, eltype, k, what=""):
+    """`close`, and FLUSH beside it."""
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    ok = np.abs(got - want) <= FLUSH
+    ref.close(np.where(ok, want, got), want, mag, eltype, k, what)
+
+
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+@pytest.mark.parametrize("eltype", ["Float32", "BFloat16"])
+@pytest.mark.parametrize("D", [1000, 1001, 4400])
+def test_norm_far_gates(cuda, far_sig, D, eltype, act):
+    """Gates from -110 to 110 (e^110 is beyond Float32), infinite ones where the activation is finite."""
+    r, T = gen(D), 16
+    gate = r.permutation(np.linspace(-110, 110, T * D)).reshape(T, D)
+    if act == "sigmoid":
+        gate[3, 5:9] = [np.inf, -np.inf, np.inf, -np.inf]
+    gt, gv = dev(gate, eltype)
+    R, Rv = dev(r.standard_normal((T, D)))
+    h, hv = dev(r.standard_normal((T, D)), eltype)
+    w, wv = dev(1 + 0.1 * r.standard_normal(D))
+    hw, hwv = dev(1 + 0.1 * r.standard_normal(D))
+    dy, dyv = dev(r.standard_normal((T, D)), eltype)
+    dro, drov = dev(r.standard_normal((T, D)))
+    y, ro = out((T, D), eltype), out((T, D))
+    mk.block_norm(y, ro, R, w, h=h, hw=hw, gate=gt, act=act)
+    g = {"r": out((T, D)), "w": out((D,)), "h": out((T, D), eltype), "hw": out((D,)), "gate": out((T, D), eltype)}
+    mk.block_norm_grad(g["r"], g["w"], dy, R, w, drout=dro, h=h, dh=g["h"], hw=hw, dhw=g["hw"], gate=gt,
+                       dgate=g["gate"], act=act)
+    mk.synchronize(BE)
+    wy, wro, want = ref.norm(Rv, wv, hv, hwv, gv, act, None, 1e-5, dy=dyv, drout=drov)
+    term, k = np.abs(Rv) + np.abs(wro - Rv), 64 + D / 64
+    # 16-bit gates: the exponent's rounding adds 110 units
+    k += 110 if eltype != "Float32" else 0
+    rms = 1 / np.sqrt((wro**2).mean(-1, keepdims=True) + 1e-5)
+    near(host(ro), wro, term, "Float32", k, "rout")
+    near(host(y), wy, term * rms * np.abs(wv) + np.abs(wy) * (1 + (term**2).mean(-1, keepdims=True) * rms**2), eltype,
+         k, "y")
+    for name, x in g.items():  # errors are relative to a column's largest value, as in test_norm; rout reaches 110 |n|
+        top = (np.abs(want[name]).max(-1, keepdims=True) + 1.0) * np.ones_like(want[name])
+        token = name in ("r", "h", "gate")
+        near(host(x), want[name], top * (1 + np.abs(term).max()), "Float32" if name == "r" or not token else eltype,
+             k * (1 if token else 1 + T / 8), (act, "d" + name))
+
+
+@pytest.mark.parametrize("eltype", ["Float32", "BFloat16"])
+@pytest.mark.parametrize("D", [64, 33])
+def test_conv_far_inputs(cuda, far_sig, D, eltype):
+    """Values in front of the silu from -110 to 110.  Their own W + 1 roundings move it by up to 111 times as much."""
+    r, T, W = gen(D), 200, 2
+    x, xv = dev(r.permutation(np.linspace(-88, 88, T * D)).reshape(T, D), eltype)
+    w, wv = dev(np.stack([np.full(D, 0.25), np.ones(D)]))
+    dy, dyv = dev(r.standard_normal((T, D)), eltype)
+    y, dx, dw = out((T, D), eltype), out((T, D), eltype), out((W, D))
+    mk.causal_conv(y, x, w)
+    mk.causal_conv_grad(dx, dw, dy, x, w)
+    st, y1 = out((T, W - 1, D), eltype, 0.0), out((T, D), eltype)
+    mk.causal_conv_step(y1, st, st, x, w)
+    mk.synchronize(BE)
+    a = (xv, wv, np.zeros(D), True, [(0, T)], None, dyv)
+    want, mag, k = ref.conv(*a), ref.conv(*a, mag=True), 64 + 3 * 111 + 110
+    near(host(y), want[0], mag[0], eltype, k, "y")
+    near(host(dx), want[2], mag[2], eltype, k, "dx")
+    near(host(dw), want[3], mag[3], "Float32", k + T / 8, "dw")
+    a = (xv, wv, np.zeros(D), True, ref.spans_of([1] * T))
+    near(host(y1), ref.conv(*a)[0], ref.conv(*a, mag=True)[0], eltype, k, "step")
+
+
+@pytest.mark.parametrize("eltype", ["Float32", "BFloat16"])
+@pytest.mark.parametrize("D", [64, 33])
+def test_scan_far_gates(cuda, far_sig, D, eltype):
+    """Gates from -110 to 110, in whole sequences, pieces and single tokens."""
+    for lens in ([40] * 5, [640]):
+        c = scan_case(lens, D, 16, 1, 0, 0, True, True, True, True, True, eltype)
+        c["z"], c["v"]["z"] = dev(gen(D).permutation(np.linspace(-110, 110, c["T"] * D)).reshape(c["T"], D), eltype)
+        saved = mk.selective_scan_saved(c["u"], c["A"], seqs=seqs_of(c["spans"]))
+        y, _ = scan_forward(c, saved)
+        g = scan_grad(c, saved)
+        mk.synchronize(BE)
+        (wy, _, want), (my, _, mag) = scan_ref(c, True), scan_ref(c, True, True)
+        k = k_scan(c) + 110
+        near(host(y), wy, my, eltype, k, "y")
+        for name in ("u", "delta", "z", "B", "C"):
+            near(host(g[name]), want[name], mag[name], eltype, k, "d" + name)
+        for name in ("A", "D", "bias", "init"):
+            near(host(g[name]), want[name], mag[name], "Float32", k + c["T"] / 8, "d" + name)
+    c = scan_case([1] * 60, D, 16, 1, 0, 0, True, True, True, True, True, eltype)
+    c["z"], c["v"]["z"] = dev(gen(D).permutation(np.linspace(-110, 110, 60 * D)).reshape(60, D), eltype)
+    y, nxt = out((60, D), eltype), out((60, D, 16))
+    mk.selective_scan_step(y, nxt, c["init"], c["u"], c["delta"], c["A"], c["B"], c["C"], D=c["skip"], z=c["z"],
+                           bias=c["bias"])
+    mk.synchronize(BE)
+    near(host(y), scan_ref(c)[0], scan_ref(c, mag=True)[0], eltype, k_scan(c) + 110, "step")

@@ -371,9 +371,10 @@ def _norm(call: _Call, r, w, h, hw, gate, scale, act, eps, lead):
         _fail(call.what, f"`r` has element type {rt}, expected Float32 or {call.eltype}")
     if h is None and not (gate is None and hw is None and scale is None):
         _fail(call.what, "`gate`, `hw` and `scale` belong to `h`")
-    pr, ldr = call.tokens(r, "r", eltype=rt)
-    dims = r.dims
+    # the sizes of the call are those of its first array, which the others are compared with
+    dims = lead.dims
     D, T = dims[0], dims[1] if len(dims) == 2 else math.prod(dims[1:])
+    pr, ldr = call.tokens(r, "r", D, T, eltype=rt)
     ph, pg, ldh, ldg = call.like("h gate", D, T, h, gate)
     phw, psc, pw = call.floats("hw scale w", D, hw, scale, w)
     # fields in the struct's order, up to ldgate

@@ -223,3 +223,42 @@ def test_plain_gradients_against_differences():
             return ref.norm(*a, dy=dy, drout=dro)[2] if grad else sum(
                 (x * g).sum() for x, g in zip(ref.norm(*a), (dy, dro)))
         check(n, run_norm)
+
+
+def refused(monkeypatch, cases):
+    """Every call raises with its message, and none comes as far as a launch."""
+    launched = []
+    monkeypatch.setattr(mk.statespace, "launch", lambda *a: launched.append(a[3]))
+    for call, msg in cases:
+        with pytest.raises(mk.MLIRKernelsError, match=msg):
+            call()
+    assert not launched
+
+
+def test_norm_arrays_of_other_sizes_are_refused(monkeypatch):
+    """Arrays that agree with one another, but not with r."""
+    y, h, g, w = fake((8, 16)), fake((8, 16)), fake((8, 16)), fake((8,))
+    longer, wider = fake((8, 32)), fake((16, 16))
+    refused(monkeypatch, [
+        (lambda: mk.block_norm(y, None, longer, w, h=h), "expected 8 x 16"),
+        (lambda: mk.block_norm(y, None, longer, w), "expected 8 x 16"),
+        (lambda: mk.block_norm(None, fake((8, 32)), longer, None, h=h), "expected 8 x 16"),
+        (lambda: mk.block_norm(None, y, longer, None), "expected 8 x 32"),
+        (lambda: mk.block_norm(None, y, longer, None, h=h), "expected 8 x 16"),
+        (lambda: mk.block_norm(None, longer, y, None, h=h), "expected 8 x 16"),
+        (lambda: mk.block_norm(None, fake((16, 16)), wider, None, h=h), "expected 8 x 16"),
+        (lambda: mk.block_norm(y, None, wider, fake((16,)), h=h), "expected 8 x 16"),
+        (lambda: mk.block_norm(y, None, longer, w, h=longer, gate=g), "expected 8 x 32"),
+        (lambda: mk.block_norm(y, None, mk.rows(fake((9, 32)), 1, 8), w, h=h), "expected 8 x 16"),
+        (lambda: mk.block_norm(mk.rows(fake((9, 16)), 1, 8), None, longer, w), "expected 8 x 16"),
+        (lambda: mk.block_norm(fake((8,)), None, y, w), "expected 8 x 1"),
+        (lambda: mk.block_norm_grad(longer, w, y, longer, w), "expected 8 x 16"),
+        (lambda: mk.block_norm_grad(longer, w, y, longer, w, h=h, dh=g), "expected 8 x 16"),
+        (lambda: mk.block_norm_grad(longer, w, longer, longer, w, h=h, dh=g), "expected 8 x 16"),
+        (lambda: mk.block_norm_grad(y, w, y, y, w, h=h, dh=longer), "expected 8 x 16"),
+        (lambda: mk.block_norm_grad(longer, w, y, y, w, h=h, dh=g), "expected 8 x 16"),
+        (lambda: mk.block_norm_grad(longer, None, None, longer, None, drout=y), "expected 8 x 32"),
+        (lambda: mk.block_norm_grad(longer, None, None, longer, None, drout=longer, h=h, dh=g), "expected 8 x 16"),
+        (lambda: mk.block_norm_grad(fake((16, 16)), None, None, wider, None, drout=fake((16, 16)), h=h, dh=g),
+         "expected 8 x 16"),
+    ])

@@ -53,9 +53,11 @@ class _Call:
 
     def tokens(self, a, name: str, rows: int | None = None, cols: int | None = None, eltype: str | None = None):
         """A token array as (pointer, ld); its element type is the call's unless given."""
-        if type(a) is MLIRArray and a.dims == self.lead and a.eltype == (eltype or self.eltype):
-            self.arrays.append(a)  # like the call's first array
-            return a.storage.data_ptr(), a.dims[0]
+        dims = self.lead
+        if (type(a) is MLIRArray and a.dims == dims and (rows is None or rows == dims[0])
+                and a.eltype == (eltype or self.eltype)):
+            self.arrays.append(a)  # like the call's first array, whose tokens all others have
+            return a.storage.data_ptr(), dims[0]
         if not isinstance(a, (MLIRArray, MLIRRows)):
             _fail(self.what, f"`{name}` must be an MLIRArray or rows of one, got {type(a).__name__}")
         if a.eltype not in _FLOATS:
@@ -248,9 +250,9 @@ def _states(call: _Call, A, B, D: int, T: int):
     if A is None or len(A.dims) != 2 or A.dims[1] != D:
         _fail(call.what, f"`A` must be (states, {D})")
     N = A.dims[0]
-    rows = math.prod(B.dims) // T if T and isinstance(B, (MLIRArray, MLIRRows)) else N
+    rows, rest = divmod(math.prod(B.dims), T) if T and isinstance(B, (MLIRArray, MLIRRows)) else (N, 0)
     G = rows // N if N else 0
-    if G < 1 or D % G:
+    if G < 1 or D % G or rest or rows % N:
         _fail(call.what, f"`B` has dims {getattr(B, 'dims', None)}: not (groups of) {N} rows for {T} tokens")
     return p, N, G
 

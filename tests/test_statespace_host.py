@@ -262,3 +262,34 @@ def test_norm_arrays_of_other_sizes_are_refused(monkeypatch):
         (lambda: mk.block_norm_grad(fake((16, 16)), None, None, wider, None, drout=fake((16, 16)), h=h, dh=g),
          "expected 8 x 16"),
     ])
+
+
+def test_scan_matrices_of_other_rows_are_refused(monkeypatch):
+    """B, C and their gradients with as many rows as u has channels, where the call needs another number."""
+    u, x, A, B = fake((8, 16)), fake((8, 16)), fake((4, 8)), fake((4, 16))
+    saved = fake((4, 8, 1))
+    refused(monkeypatch, [
+        (lambda: mk.selective_scan(x, u, u, A, B, u), "`C` has dims"),
+        (lambda: mk.selective_scan(x, u, u, A, u, B), "`C` has dims"),
+        (lambda: mk.selective_scan(x, u, u, fake((3, 8)), u, u), "`B` has dims"),
+        (lambda: mk.selective_scan(x, u, u, fake((16, 8)), fake((16, 16)), u), "`C` has dims"),
+        (lambda: mk.selective_scan(x, u, u, A, fake((6, 16)), fake((6, 16))), "`B` has dims"),
+        (lambda: mk.selective_scan(x, u, u, A, fake((4, 17)), fake((4, 17))), "`B` has dims"),
+        (lambda: mk.selective_scan_step(x, fake((4, 8, 16)), fake((4, 8, 16)), u, u, A, B, u), "`C` has dims"),
+        (lambda: mk.selective_scan_step(x, fake((3, 8, 16)), fake((3, 8, 16)), u, u, fake((3, 8)), u, u),
+         "`B` has dims"),
+        (lambda: mk.selective_scan_grad(x, x, A, x, B, u, u, u, A, B, B, saved), "`dB` has dims"),
+        (lambda: mk.selective_scan_grad(x, x, A, B, x, u, u, u, A, B, B, saved), "`dC` has dims"),
+        (lambda: mk.selective_scan_grad(x, x, A, fake((8, 16)), fake((8, 16)), u, u, u, A, B, B, saved), "`dB` has"),
+    ])
+
+
+def test_scan_matrices_of_as_many_rows_as_channels(monkeypatch):
+    """The same number of rows where it is the right one: N states, or groups of them."""
+    seen = []
+    monkeypatch.setattr(mk.statespace, "launch", lambda entry, args, arrays, what: seen.append(args))
+    u, x = fake((8, 16)), fake((8, 16))
+    for A, G in ((fake((8, 8)), 1), (fake((4, 8)), 2), (fake((2, 8)), 4)):
+        mk.selective_scan(x, u, u, A, fake((8, 16)), u)
+        mk.selective_scan(x, u, u, A, mk.rows(fake((9, 16)), 2, 9), fake((8 // G, G, 16)))
+        assert [(a.N, a.G, a.ldb, a.ldc) for a in seen[-2:]] == [(8 // G, G, 8, 8), (8 // G, G, 9, 8)]

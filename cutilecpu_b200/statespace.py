@@ -65,7 +65,7 @@ class _Call:
         dims = a.dims
         if self.eltype is None:
             self.eltype = a.eltype
-        if self.lead is None and len(dims) > 1:
+        if self.lead is None:
             self.lead = dims
         if a.eltype != (eltype or self.eltype):
             _fail(self.what, f"`{name}` has element type {a.eltype}, expected {eltype or self.eltype}")

@@ -293,3 +293,21 @@ def test_scan_matrices_of_as_many_rows_as_channels(monkeypatch):
         mk.selective_scan(x, u, u, A, fake((8, 16)), u)
         mk.selective_scan(x, u, u, A, mk.rows(fake((9, 16)), 2, 9), fake((8 // G, G, 16)))
         assert [(a.N, a.G, a.ldb, a.ldc) for a in seen[-2:]] == [(8 // G, G, 8, 8), (8 // G, G, 9, 8)]
+
+
+def test_one_token_without_a_second_dimension(monkeypatch):
+    """u of one dimension is one token; the others are compared with it, not with the first matrix that follows."""
+    u, A, B, st = fake((8,)), fake((4, 8)), fake((4, 1)), fake((4, 8, 1))
+    refused(monkeypatch, [
+        (lambda: mk.selective_scan_step(fake((4, 1)), st, st, u, u, A, B, B), "`y` has dims"),
+        (lambda: mk.selective_scan_step(u, st, st, u, fake((4, 1)), A, B, B), "`delta` has dims"),
+        (lambda: mk.selective_scan(fake((4, 1)), u, u, A, B, B), "`y` has dims"),
+        (lambda: mk.selective_scan_grad(fake((4, 1)), u, A, B, B, u, u, u, A, B, B, st), "`du` has dims"),
+        (lambda: mk.causal_conv(fake((4, 1)), u, fake((8, 4))), "`y` has dims"),
+    ])
+    seen = []
+    monkeypatch.setattr(mk.statespace, "launch", lambda entry, args, arrays, what: seen.append(args))
+    mk.selective_scan_step(u, st, st, u, fake((8, 1)), A, B, fake((4, 1, 1)), z=u)
+    mk.causal_conv_step(u, fake((8, 3, 1)), fake((8, 3, 1)), u, fake((8, 4)))
+    mk.block_norm(u, None, fake((8, 1)), fake((8,)), h=u)
+    assert [(a.D, a.T if hasattr(a, "T") else a.B) for a in seen] == [(8, 1)] * 3

@@ -152,7 +152,10 @@ class _Call:
             return None, 0
         if first is not None and second is not None and first != second:
             _fail(self.what, f"the state pools hold different numbers of states: {sorted((first, second))}")
-        return self.dense(slots, "slots", count, "Int32"), second if first is None else first
+        p = self.dense(slots, "slots", count, "Int32")
+        if first is None and second is None:
+            _fail(self.what, "`slots` without `init` or `last`, whose columns they choose")
+        return p, second if first is None else first
 
     def run(self, entry: str, args, workspace: str | None = None):
         L = _lib.lib()

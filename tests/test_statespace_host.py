@@ -311,3 +311,11 @@ def test_one_token_without_a_second_dimension(monkeypatch):
     mk.causal_conv_step(u, fake((8, 3, 1)), fake((8, 3, 1)), u, fake((8, 4)))
     mk.block_norm(u, None, fake((8, 1)), fake((8,)), h=u)
     assert [(a.D, a.T if hasattr(a, "T") else a.B) for a in seen] == [(8, 1)] * 3
+
+
+def test_slots_without_a_pool_are_refused(monkeypatch):
+    x, A, B, one = fake((8, 16)), fake((4, 8)), fake((4, 16)), fake((1,), "Int32")
+    refused(monkeypatch, [
+        (lambda: mk.causal_conv(fake((8, 16)), x, fake((8, 4)), slots=one), "`slots` without"),
+        (lambda: mk.selective_scan(fake((8, 16)), x, x, A, B, B, slots=one), "`slots` without"),
+    ])

@@ -253,7 +253,12 @@ def _states(call: _Call, A, B, D: int, T: int):
     if A is None or len(A.dims) != 2 or A.dims[1] != D:
         _fail(call.what, f"`A` must be (states, {D})")
     N = A.dims[0]
-    rows, rest = divmod(math.prod(B.dims), T) if T and isinstance(B, (MLIRArray, MLIRRows)) else (N, 0)
+    rows, rest = N, 0
+    if isinstance(B, (MLIRArray, MLIRRows)) and B.dims:
+        if T:
+            rows, rest = divmod(math.prod(B.dims), T)
+        else:  # (N, G, no tokens) has one dimension more than u
+            rows = math.prod(B.dims[:2 if len(B.dims) > len(call.lead) else 1])
     G = rows // N if N else 0
     if G < 1 or D % G or rest or rows % N:
         _fail(call.what, f"`B` has dims {getattr(B, 'dims', None)}: not (groups of) {N} rows for {T} tokens")

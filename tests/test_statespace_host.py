@@ -319,3 +319,19 @@ def test_slots_without_a_pool_are_refused(monkeypatch):
         (lambda: mk.causal_conv(fake((8, 16)), x, fake((8, 4)), slots=one), "`slots` without"),
         (lambda: mk.selective_scan(fake((8, 16)), x, x, A, B, B, slots=one), "`slots` without"),
     ])
+
+
+def test_no_tokens_with_groups_as_rows(monkeypatch):
+    """No tokens: B and C as rows of a wider matrix have the rows of all groups, as they have with tokens."""
+    seen = []
+    monkeypatch.setattr(mk.statespace, "launch", lambda entry, args, arrays, what: seen.append(args))
+    u, A = fake((8, 0)), fake((4, 8))
+    for B in (fake((8, 0)), mk.rows(fake((9, 0)), 2, 9), fake((4, 2, 0)), fake((4, 0))):
+        mk.selective_scan(fake((8, 0)), u, u, A, B, B, seqs=fake((1,), "Int32"))
+        mk.selective_scan_step(fake((8, 0)), fake((4, 8, 0)), fake((4, 8, 0)), u, u, A, B, B)
+    assert [(a.G, a.N) for a in seen] == [(2, 4)] * 6 + [(1, 4)] * 2
+    refused(monkeypatch, [
+        (lambda: mk.selective_scan(fake((8, 0)), u, u, A, fake((6, 0)), fake((6, 0))), "`B` has dims"),
+        (lambda: mk.selective_scan(fake((8, 0)), u, u, A, fake((8, 0)), fake((4, 0))), "`C` has dims"),
+        (lambda: mk.selective_scan(fake((8, 0)), u, u, A, None, fake((4, 0))), "`B` "),
+    ])

@@ -109,11 +109,21 @@ __device__ __forceinline__ void reduce_states(float (&v)[CH][K], int p, float (&
   reduce_scatter<K, P / CH, CW * CH>(v[0], p / CH, out);
 }
 
+// Looks sequence i over: its offsets and its slot.  There are at least as many
+// items as sequences, so that item i does this for sequence i, whichever
+// sequence it is a piece of: where offsets descend, some have no item at all.
+template <typename T>
+__device__ __forceinline__ void check_sequence(const Scan<T>& p, int64_t i) {
+  if (i >= p.q.nseq) return;
+  if (threadIdx.x == 0 && seq_span(p.q, i).bad) atomicOr(p.err, mk::ERRBIT_SEQS);
+  check_distinct(p.slots, i, threadIdx.x, kThreads, p.err);
+}
+
 struct Item {
   int64_t s, c, first;  // sequence, piece of it, number of its first piece
   int64_t lo, hi;       // the sequence's columns
   int64_t t0, t1;       // the piece's
-  bool bad, none;       // none: no such piece
+  bool none;            // no such piece
 };
 
 template <typename T>
@@ -123,7 +133,6 @@ __device__ __forceinline__ Item item_at(const Scan<T>& p, int64_t i) {
   it.first = p.piece ? first_piece(p.q, it.s, p.piece) : i;
   it.c = i - it.first;
   const Span sp = seq_span(p.q, it.s);
-  it.bad = sp.bad;
   it.lo = sp.lo;
   it.hi = sp.hi;
   it.t0 = sp.lo + it.c * p.piece;
@@ -369,13 +378,10 @@ __global__ void __launch_bounds__(kThreads, NS <= 4 ? 4 : 3) scan_fwd(Scan<T> p)
   __shared__ __align__(16) float sC[FULL ? kTS : 1][NP];
   const int64_t tile = blockIdx.x % p.tiles, item = blockIdx.x / p.tiles;
   const W w = place<NS, P, CH>(p, tile);
+  if (FULL && tile == 0) check_sequence(p, item);
   const Item it = item_at(p, item);
   if (it.none) return;
   const int64_t n0 = w.p * NS;
-  if (FULL && tile == 0 && it.c == 0) {
-    if (threadIdx.x == 0 && it.bad) atomicOr(p.err, mk::ERRBIT_SEQS);
-    check_distinct(p.slots, it.s, threadIdx.x, kThreads, p.err);
-  }
   const int64_t row = p.init || p.last ? slot_of(p.slots, p.nslots, it.s, p.err) : -1;
 
   RawFwd<T, V, S::NV> cur, nxt;
@@ -824,9 +830,9 @@ __global__ void __launch_bounds__(kThreads, CH == 1 && NS <= 4 ? 4 : NS == 2 ? 3
   };
 
   for (int64_t item = item0; item < p.items; item += p.grid_items) {
+    if (tile == 0) check_sequence(p, item);
     const Item it = item_at(p, item);
     if (it.none) continue;
-    if (tile == 0 && it.c == 0 && threadIdx.x == 0 && it.bad) atomicOr(p.err, mk::ERRBIT_SEQS);
     F2 e_[CH][H];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {

@@ -20,7 +20,7 @@ are taken from and put into that column of a pool; entries <= 0 have no state
 
 Offsets and slots are read on the device.  Bad ones (offsets that descend or
 leave the array, slots above the pool or used twice) raise ``KernelException``
-at the next ``synchronize``.
+at the next ``synchronize``; results of such a call are not to be used.
 
 A gradient overwrites the arrays given for it.  Workspaces come from torch's
 allocator, so a call may be captured into a CUDA graph; two graphs do not share

@@ -311,7 +311,9 @@ MK_API int mk_peer_trace(unsigned long long* log_dev, int entries);
  * sequences are neither read nor written.  With seqs == NULL every sequence
  * has `len` columns and nseq * len == T.  A sequence may be empty; its state
  * passes through.  Offsets that descend or leave the T columns make that
- * sequence empty and set the device error word (mk_error_poll).
+ * sequence empty and set the device error word (mk_error_poll); where they
+ * descend, sequences may overlap, and what the call leaves of the others is
+ * undefined (nothing outside the arrays is touched).
  * Slots: with slots (one 1-BASED Int32 per sequence or batch entry), the
  * state of entry i is column slots[i] of the pool; slots[i] <= 0 means none
  * (a prompt then starts from zero and leaves no state; a step's entry is

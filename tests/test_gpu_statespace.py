@@ -908,3 +908,22 @@ def test_scan_far_gates(cuda, far_sig, D, eltype):
                            bias=c["bias"])
     mk.synchronize(BE)
     near(host(y), scan_ref(c)[0], scan_ref(c, mag=True)[0], eltype, k_scan(c) + 110, "step")
+
+
+@pytest.mark.parametrize("offsets", [[1, 501, 101, 1025], [1, 1001, 20, 30, 1025], [1, 2000, 700, 1025],
+                                     [-5, 300, 200, 1025]])
+def test_bad_offsets_are_reported_in_pieces(cuda, offsets):
+    """The same where sequences are cut: every offset is looked at, whichever sequence a piece is taken for."""
+    c = scan_case([1024], 20, 16, 1, 0, 0, True, True, True, True, False, "Float32")
+    bad, S = ints(offsets), len(offsets) - 1
+    saved = mk.selective_scan_saved(c["u"], c["A"], seqs=bad)
+    saved.storage.zero_()
+    y, last = out((1024, 20)), out((S, 20, 16))
+    mk.selective_scan(y, c["u"], c["delta"], c["A"], c["B"], c["C"], seqs=bad, last=last, saved=saved)
+    with pytest.raises(mk.KernelException, match="offsets"):
+        mk.synchronize(BE)
+    du, dd, dA, dB, dC = (out(s) for s in ((1024, 20), (1024, 20), (20, 16), (1024, 16), (1024, 16)))
+    mk.selective_scan_grad(du, dd, dA, dB, dC, c["dy"], c["u"], c["delta"], c["A"], c["B"], c["C"], saved, seqs=bad)
+    with pytest.raises(mk.KernelException, match="offsets"):
+        mk.synchronize(BE)
+    mk.synchronize(BE)

@@ -927,3 +927,40 @@ def test_bad_offsets_are_reported_in_pieces(cuda, offsets):
     with pytest.raises(mk.KernelException, match="offsets"):
         mk.synchronize(BE)
     mk.synchronize(BE)
+
+
+@pytest.mark.parametrize("eltype,D", [("Float32", 33), ("Float32", 96), ("BFloat16", 96), ("BFloat16", 33),
+                                      ("BFloat16", 4104), ("Float32", 4104), ("BFloat16", 8200)])
+def test_norm_gradient_of_absent_parts(cuda, D, eltype):
+    """Without dy the norm of rout takes no part: infinite and undefined values of r stay out of the gradients.
+    Without hw that of h does not: neither do infinite values of h."""
+    r, T = gen(D), 5
+    Rv = r.standard_normal((T, D))
+    Rv[1, ::7], Rv[2, ::5], Rv[3, 0] = np.inf, -np.inf, np.nan
+    R, _ = dev(Rv)
+    h, hv = dev(r.standard_normal((T, D)), eltype)
+    gt, gv = dev(r.standard_normal((T, D)), eltype)
+    hw, hwv = dev(1 + 0.1 * r.standard_normal(D))
+    sc, scv = dev(r.standard_normal(D))
+    dro, drov = dev(r.standard_normal((T, D)))
+    dr = out((T, D))
+    mk.block_norm_grad(dr, None, None, R, None, drout=dro)
+    mk.synchronize(BE)
+    np.testing.assert_array_equal(host(dr), drov)
+    dr, dh, dhw, dg, ds = out((T, D)), out((T, D), eltype), out((D,)), out((T, D), eltype), out((D,))
+    mk.block_norm_grad(dr, None, None, R, None, drout=dro, h=h, dh=dh, hw=hw, dhw=dhw, gate=gt, dgate=dg, scale=sc,
+                       dscale=ds)
+    mk.synchronize(BE)
+    np.testing.assert_array_equal(host(dr), drov)
+    want = ref.norm(np.zeros((T, D)), None, hv, hwv, gv, "silu", scv, 1e-5, drout=drov)[2]
+    for name, x in (("h", dh), ("hw", dhw), ("gate", dg), ("scale", ds)):
+        top = (np.abs(want[name]).max(-1, keepdims=True) + 1.0) * np.ones_like(want[name])
+        ref.close(host(x), want[name], top, eltype if name in ("h", "gate") else "Float32", (64 + D / 64) * (1 + T / 8),
+                  name)
+    hv[0, ::3], hv[4, -1] = np.inf, -np.inf
+    h, _ = dev(hv, eltype)
+    dr, dh = out((T, D)), out((T, D), eltype)
+    mk.block_norm_grad(dr, None, None, R, None, drout=dro, h=h, dh=dh)
+    mk.synchronize(BE)
+    np.testing.assert_array_equal(host(dr), drov)
+    ref.close(host(dh), drov, np.abs(drov), eltype, 4, "dh without hw")

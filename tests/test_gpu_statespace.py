@@ -964,3 +964,38 @@ def test_norm_gradient_of_absent_parts(cuda, D, eltype):
     mk.synchronize(BE)
     np.testing.assert_array_equal(host(dr), drov)
     ref.close(host(dh), drov, np.abs(drov), eltype, 4, "dh without hw")
+
+
+@pytest.mark.parametrize("eltype", list(TD))
+@pytest.mark.parametrize("B,D,N,G", [(80, 516, 16, 1), (60, 700, 8, 1), (75, 520, 7, 2), (100, 390, 24, 3),
+                                     (60, 660, 13, 1), (60, 520, 64, 1), (70, 640, 3, 1)])
+def test_scan_step_of_a_serving_batch(cuda, B, D, N, G, eltype):
+    """Enough entries and channels for several channels per thread, the last of a tile beyond the group's end."""
+    test_scan_step(cuda, B, D, N, G, eltype)
+
+
+@pytest.mark.parametrize("D,N,G,eltype", [(4096, 16, 32, "BFloat16"), (4096, 7, 32, "Float16"), (4096, 24, 32, "BFloat16"),
+                                          (4096, 16, 32, "Float32"), (4095, 16, 35, "BFloat16"), (2048, 64, 16, "Float16")])
+def test_gradients_of_many_sequences(cuda, D, N, G, eltype):
+    """Several sequences for each block of the gradient, two channels per lane or one; the first and the last group
+    are compared."""
+    lens = [int(n) for n in gen(D + N).integers(0, 40, 80)]
+    c = scan_case(lens, D, N, G, 1, 2, True, True, True, True, True, eltype)
+    saved = mk.selective_scan_saved(c["u"], c["A"], seqs=seqs_of(c["spans"]))
+    y, last = scan_forward(c, saved)
+    g = scan_grad(c, saved)
+    mk.synchronize(BE)
+    ch, gr, m = np.r_[:D // G, D - D // G:D], [0, G - 1], inside(c["spans"], c["T"])
+    v = c["v"]
+    sub = dict(c, D=2 * (D // G), v={k: v[k][:, ch] for k in ("u", "delta", "z", "dy", "init", "dlast")}
+               | {k: v[k][ch] for k in ("A", "skip", "bias")} | {k: v[k][:, gr] for k in ("B", "C")})
+    (wy, wl, wg), (my, ml, mg) = scan_ref(sub, True), scan_ref(sub, True, True)
+    ref.close(host(y)[m][:, ch], wy[m], my[m], eltype, k_scan(c))
+    ref.close(host(last)[:, ch], wl, ml, "Float32", k_scan(c))
+    for name in ("u", "delta", "z"):
+        ref.close(host(g[name])[m][:, ch], wg[name][m], mg[name][m], eltype, k_scan(c), name)
+    for name in ("B", "C"):
+        ref.close(host(g[name])[m][:, gr], wg[name][m], mg[name][m], eltype, k_scan(c), name)
+    for name in ("A", "D", "bias"):
+        ref.close(host(g[name])[ch], wg[name], mg[name], "Float32", k_scan(c) + c["T"] / 8, name)
+    ref.close(host(g["init"])[:, ch], wg["init"], mg["init"], "Float32", k_scan(c) + c["T"] / 8, "init")

@@ -185,7 +185,10 @@ int check_scan(const char* who, const mk_scan_args* a, bool grad) {
 // from 1.5 of their blocks per SM on, and in pieces where the blocks that an SM
 // holds (two) get 512 tokens each (4 x 2048 of 2048 457 -> 417 us; 1 x 8192 of
 // 1024, 443 tokens, 235 -> 254 us).  Single elements take registers that two
-// channels need (4 x 2048 x 4095 1273 -> 1302 us): one.
+// channels need (4 x 2048 x 4095 1273 -> 1302 us), and so does Float32 beside 2
+// states per lane (8 states, 4 x 2048 tokens of 4096 channels whole 825 -> 1060 us,
+// 16 x 1024 1439 -> 1729; in bf16 two win there, 771 -> 750 us, and in Float32
+// with 16 states, 1189 -> 1073): one.
 Plan plan(const mk_scan_args* a, const mk::Device* dev, bool grad) {
   Plan b{};
   const int64_t Dg = a->D / a->G, sms = dev->sms, CB = kWarps * (32 / lanes_of(a->N));
@@ -195,7 +198,7 @@ Plan plan(const mk_scan_args* a, const mk::Device* dev, bool grad) {
   const bool cut = have > 0 && a->T >= a->nseq * 4 * kTS &&
                    (grad ? have <= sms * (a->seqs ? 6 : 3) : have * 3 <= 4 * sms);
   b.ch = 1;
-  if (grad && a->N <= 16 && all_vec(a, true)) {  // the registers hold no two channels of 8 states
+  if (grad && two_channels(states_of(a->N), type_bytes(a->type)) && all_vec(a, true)) {
     const bool enough = cut ? twice * a->T >= 2 * sms * 512 : 2 * twice * a->nseq >= 3 * sms;
     if (enough) b.ch = 2;
   }

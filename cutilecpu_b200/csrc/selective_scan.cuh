@@ -1155,6 +1155,9 @@ __global__ void __launch_bounds__(256) scan_fold(Scan<T> p, T* dB, T* dC, int64_
 // Lanes per channel and states per lane: 2, 4 or 8 states on 4 lanes, beyond 32 states 8 on 8.
 inline int lanes_of(int64_t N) { return N <= 32 ? 4 : 8; }
 inline int states_of(int64_t N) { return N <= 8 ? 2 : N <= 16 ? 4 : 8; }
+// Whether the gradient's registers hold two channels per lane: not with 8 states,
+// nor with Float32 and 2 states (the code for it spilled 576 bytes).
+constexpr bool two_channels(int states, size_t type_size) { return states == 4 || (states == 2 && type_size == 2); }
 
 // Whether the token matrices can be taken in vectors of 16 bytes.
 inline bool all_vec(const mk_scan_args* a, bool grad) {
@@ -1249,7 +1252,7 @@ template <typename T, int NS, int P>
 int run_vec(const mk_scan_args* a, const mk::Device* dev, const Plan& b, bool grad, cudaStream_t s) {
   const bool vec = all_vec(a, grad);
   if (!grad) return vec ? run_fwd<T, NS, P, true>(a, dev, b, s) : run_fwd<T, NS, P, false>(a, dev, b, s);
-  if constexpr (NS <= 4) {
+  if constexpr (two_channels(NS, sizeof(T))) {
     if (b.ch == 2) return run_bwd<T, NS, P, 2, true>(a, dev, b, s);
   }
   return vec ? run_bwd<T, NS, P, 1, true>(a, dev, b, s) : run_bwd<T, NS, P, 1, false>(a, dev, b, s);

@@ -975,7 +975,8 @@ def test_scan_step_of_a_serving_batch(cuda, B, D, N, G, eltype):
 
 
 @pytest.mark.parametrize("D,N,G,eltype", [(4096, 16, 32, "BFloat16"), (4096, 7, 32, "Float16"), (4096, 24, 32, "BFloat16"),
-                                          (4096, 16, 32, "Float32"), (4095, 16, 35, "BFloat16"), (2048, 64, 16, "Float16")])
+                                          (4096, 16, 32, "Float32"), (4096, 7, 32, "Float32"),
+                                          (4095, 16, 35, "BFloat16"), (2048, 64, 16, "Float16")])
 def test_gradients_of_many_sequences(cuda, D, N, G, eltype):
     """Several sequences for each block of the gradient, two channels per lane or one; the first and the last group
     are compared."""

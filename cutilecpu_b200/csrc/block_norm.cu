@@ -641,8 +641,9 @@ int run_fwd(const mk_norm_args* a, cudaStream_t s) {
 }
 
 // Values per thread: 8, and 16 of columns beyond 4096 channels; up to 8192 of
-// them that is 512 threads, which have registers for it (4096 x 8192 bf16 630 -> 305
-// us against code for 1024, 5120 channels 458 -> 219).  Wider ones spill.
+// them that is 512 threads of 128 registers each (4096 x 8192 bf16 630 -> 305 us
+// against code for 1024, 5120 channels 458 -> 219).  They spill all the same, 220
+// to 630 bytes; beyond 8192 channels, with 64 registers, 1060 to 1860.
 struct BwdPlan {
   int V, items;
   dim3 block;

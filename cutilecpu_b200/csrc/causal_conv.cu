@@ -12,9 +12,11 @@
 //
 // bf16, 4 taps, silu, measured on B200: 16384 tokens of 4096 channels forward 55
 // us (4.9 TB/s, 0.75 of a copy; 59 us with the state pool of 7 ragged prompts),
-// 8192 x 4096 forward 29 us (4.6 TB/s), backward 57 us (3.5 TB/s: its
-// registers leave 2.5 to 4 warps to a scheduler, which use half of the issue
-// slots) and 4.3 us for conv_fold; one token of 192 entries of 4099 channels (f32, 3 taps) 5.9 us.
+// 8192 x 4096 forward 29 us (4.6 TB/s), backward 57 us (3.5 TB/s: 128
+// registers leave four warps to a scheduler, whose dependent products and waits
+// on shared memory leave half of the issue slots empty) and 4.2 us for conv_fold;
+// in Float32 50 and 93 us (conv_bwd with 4 taps spills 116 bytes there); one token
+// of 192 entries of 4099 channels (f32, 3 taps) 5.9 us.
 #include <type_traits>
 
 #include "tokens.cuh"

@@ -12,8 +12,11 @@ using namespace mk::scan;
 // takes IT channels, so that as many states are in flight and one read of B
 // and C serves them all; with IT == P each of the P lanes also computes what
 // one of those channels needs once (softplus, gate), and passes it round.  192
-// entries of 4096 channels with 16 states: 21 us, 5.0 TB/s; the copies' rate is
-// not reached because a launch this short spends 3 us starting and ending.
+// entries of 4096 channels with 16 states: 24.2 us, 4.2 TB/s, with states that are
+// not in L2 (as between two tokens of a model), 21.0 us where the call before has
+// left part of them there.  Each block waits in turn for its slot, its inputs
+// and its states (3.1 of an issue's 9 cycles are waits on global loads, 71% of the
+// issue slots are used), and 3 us go into the start and the end of the launch.
 template <typename T>
 struct Step {
   int64_t D, N, G, Dg, B, nslots, tiles, tpg;  // channel tiles, and of one group
@@ -247,8 +250,8 @@ int workspace(const char* who, const mk_scan_args* a, bool grad, size_t* bytes) 
 
 template <typename T, int P>
 int launch_step(Step<T> p, const mk::Device* dev, cudaStream_t s) {
-  // P channels per thread (up to 8): at 192 entries of 4096 channels and 16 states 47.6 -> 25.1 us, at 16 entries 6.9
-  // -> 5.3; one where fewer than two blocks per SM would be left (8 entries: 4.5 -> 4.4 us, 1 entry 3.9 -> 3.7)
+  // P channels per thread (up to 8): at 192 entries of 4096 channels and 16 states, states not in L2, 47.6 -> 25.1 us,
+  // at 16 entries 6.9 -> 5.3; one where fewer than two blocks per SM would be left (8 entries: 4.5 -> 4.4 us, 1 entry 3.9 -> 3.7)
   constexpr int IT = P <= 8 ? P : 1;
   const int64_t few = p.G * mk::cdiv(p.Dg, IT * (128 / P));
   const bool wide = few * p.B >= 2 * (int64_t)dev->sms;

@@ -22,9 +22,15 @@ Offsets and slots are read on the device.  Bad ones (offsets that descend or
 leave the array, slots above the pool or used twice) raise ``KernelException``
 at the next ``synchronize``; results of such a call are not to be used.
 
-A gradient overwrites the arrays given for it.  Workspaces come from torch's
+A gradient overwrites the arrays given for it.  Arrays that a call writes must
+not overlap its others unless it says so.  Workspaces come from torch's
 allocator, so a call may be captured into a CUDA graph; two graphs do not share
 one.
+
+Speed.  The scan and the norms take 16 bytes at a time where the channels (of a
+group), leading dimensions and first rows are multiples of that, and single
+elements otherwise, which takes 1.1 to 1.3 (scan) and 1.8 times (norms) as long:
+parts of a projection are best laid out at such multiples.
 """
 from __future__ import annotations
 
@@ -323,7 +329,9 @@ def selective_scan_grad(du, ddelta, dA, dB, dC, dy, u, delta, A, B, C, saved, *,
     """Gradients of ``selective_scan`` for ``dy`` (and ``dlast``, that of ``last``).
     ``dB`` and ``dC`` are summed over the channels of a group, ``dA``, ``dD`` and
     ``dbias`` over all tokens.  ``saved`` is what the forward pass left, for the same
-    inputs (an ``init`` is in it); ``dD``, ``dz``, ``dbias`` go with ``D``, ``z``, ``bias``."""
+    inputs (an ``init`` is in it); ``dD``, ``dz``, ``dbias`` go with ``D``, ``z``, ``bias``.
+    The workspace is 8 bytes per token, row of B and tile of 16 to 64 channels (67 MB
+    for 8192 tokens of 4096 channels with 16 states, 1.07 GB with 64)."""
     c = _Call("selective_scan_grad")
     for name, given, grad in (("D", D, dD), ("z", z, dz), ("bias", bias, dbias)):
         if (given is None) != (grad is None):

@@ -10,6 +10,7 @@ covers W + 1 products, a sigmoid and a sum over the block's tokens in registers
 and parts; sums over n tokens or channels add n / 8 (pairwise or walked by
 several threads).
 """
+import ctypes
 import itertools
 
 import numpy as np
@@ -1000,3 +1001,17 @@ def test_gradients_of_many_sequences(cuda, D, N, G, eltype):
     for name in ("A", "D", "bias"):
         ref.close(host(g[name])[ch], wg[name], mg[name], "Float32", k_scan(c) + c["T"] / 8, name)
     ref.close(host(g["init"])[:, ch], wg["init"], mg["init"], "Float32", k_scan(c) + c["T"] / 8, "init")
+
+
+def test_scan_gradient_workspace(cuda):
+    """The sums of dB and dC for every tile of channels: 8 bytes per token, row of B and tile of 32 channels (64 with
+    two per lane, 16 beyond 32 states), a few MB of parts beside them.  Only the size is asked for."""
+    p = 1 << 20  # never followed
+    for T, D, N, G, tile in ((8192, 4096, 16, 1, 64), (8192, 4096, 24, 1, 32), (8192, 4096, 64, 1, 16),
+                             (1 << 20, 8192, 16, 8, 64)):
+        a = mk._lib.ScanArgs(type=2, softplus=1, D=D, N=N, G=G, T=T, nseq=8, len=T // 8, u=p, ldu=D, delta=p, lddelta=D,
+                             dy=p, lddy=D, du=p, lddu=D, ddelta=p, ldddelta=D)
+        n = ctypes.c_size_t()
+        mk._lib.check(mk._lib.lib().mk_selective_scan_grad_workspace(a, n), "workspace")
+        sums = 8 * T * G * N * (D // G // tile)
+        assert sums <= n.value <= sums + 8 * D * (N + 2) * 4 + 1024, (T, D, N, G)

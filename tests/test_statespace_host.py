@@ -335,3 +335,52 @@ def test_no_tokens_with_groups_as_rows(monkeypatch):
         (lambda: mk.selective_scan(fake((8, 0)), u, u, A, fake((8, 0)), fake((4, 0))), "`C` has dims"),
         (lambda: mk.selective_scan(fake((8, 0)), u, u, A, None, fake((4, 0))), "`B` "),
     ])
+
+
+def every_call():
+    """The calls with all of their arrays, by name: (call, arrays)."""
+    f, i = (lambda *s: fake(s)), (lambda *s: fake(s, "Int32"))
+    D, T, S, N, G, W, P, t = 8, 16, 2, 4, 2, 3, 5, (8, 16)
+    conv = dict(x=f(*t), w=f(D, W), bias=f(D), seqs=i(S + 1))
+    scan = dict(u=f(*t), delta=f(*t), A=f(N, D), B=f(N, G, T), C=f(N, G, T), D=f(D), z=f(*t), bias=f(D), seqs=i(S + 1))
+    step = {k: v for k, v in scan.items() if k != "seqs"}
+    norm = dict(r=f(*t), w=f(D), h=f(*t), hw=f(D), gate=f(*t), scale=f(D))
+    saved = f(N, D, T // 32 + S)
+    return {
+        "causal_conv": (mk.causal_conv, dict(y=f(*t), **conv, init=f(D, W - 1, S), last=f(D, W - 1, S))),
+        "causal_conv_slots": (mk.causal_conv, dict(y=f(*t), **conv, init=f(D, W - 1, P), last=f(D, W - 1, P), slots=i(S))),
+        "causal_conv_grad": (mk.causal_conv_grad, dict(
+            dx=f(*t), dw=f(D, W), dy=f(*t), dbias=f(D), **conv, init=f(D, W - 1, S), dinit=f(D, W - 1, S),
+            dlast=f(D, W - 1, S))),
+        "causal_conv_step": (mk.causal_conv_step, dict(
+            y=f(*t), next=f(D, W - 1, T), state=f(D, W - 1, T), x=f(*t), w=f(D, W), bias=f(D))),
+        "selective_scan": (mk.selective_scan, dict(y=f(*t), **scan, init=f(N, D, S), last=f(N, D, S), saved=saved)),
+        "selective_scan_slots": (mk.selective_scan, dict(y=f(*t), **scan, init=f(N, D, P), last=f(N, D, P), slots=i(S))),
+        "selective_scan_grad": (mk.selective_scan_grad, dict(
+            du=f(*t), ddelta=f(*t), dA=f(N, D), dB=f(N, G, T), dC=f(N, G, T), dy=f(*t), **scan, saved=saved, dD=f(D),
+            dz=f(*t), dbias=f(D), dinit=f(N, D, S), dlast=f(N, D, S))),
+        "selective_scan_step": (mk.selective_scan_step, dict(y=f(*t), next=f(N, D, T), state=f(N, D, T), **step)),
+        "block_norm": (mk.block_norm, dict(y=f(*t), rout=f(*t), **norm)),
+        "block_norm_grad": (mk.block_norm_grad, dict(
+            dr=f(*t), dw=f(D), dy=f(*t), drout=f(*t), **norm, dh=f(*t), dhw=f(D), dgate=f(*t), dscale=f(D))),
+    }
+
+
+@pytest.mark.parametrize("name", list(every_call()))
+def test_every_array_of_another_size_is_refused(monkeypatch, name):
+    """One array at a time, larger or smaller in one dimension, or with dims that another array of the call has."""
+    call, arrays = every_call()[name]
+    launched = []
+    monkeypatch.setattr(mk.statespace, "launch", lambda *a: launched.append(a[3]))
+    call(**arrays)
+    assert len(launched) == 1
+    others = {a.dims for a in arrays.values() if a.eltype == "Float32"}
+    for k, a in arrays.items():
+        wrong = {a.dims[:j] + (a.dims[j] + d,) + a.dims[j + 1:] for j in range(len(a.dims)) for d in (-1, 1, a.dims[j])}
+        wrong |= {d for d in others if np.prod(d) != np.prod(a.dims)} if a.eltype == "Float32" else set()
+        if (name, k) == ("causal_conv_slots", "w"):
+            continue  # a pool is taken by its elements: it holds another number of states of other taps
+        for dims in wrong:
+            with pytest.raises(mk.MLIRKernelsError):
+                call(**dict(arrays, **{k: fake(dims, a.eltype)}))
+    assert len(launched) == 1

@@ -406,8 +406,8 @@ MK_API int mk_causal_conv_step(const mk_conv_step_args* args, void* stream);
  * dA, and those of the other inputs that are given (dz, dDskip, dbias: not
  * NULL exactly when z, Dskip, bias are; dinit optional).  Its workspace holds a
  * Float32 dB and dC for every tile of channels, 8 bytes per token, row of B and
- * tile of 64 channels (32 beyond 16 states or without 16-byte vectors, 16 beyond
- * 32 states): 67 MB for 8192 tokens, 4096 channels and 16 states, 1.07 GB for 64.
+ * tile of 64 or 32 channels (16 beyond 32 states): 67 MB for 8192 tokens, 4096
+ * channels and 16 states, 1.07 GB for 64.
  * It grows with the tokens, so a batch of sequences may be given in parts. */
 #define MK_SCAN_PIECE 32
 typedef struct mk_scan_args {
